@@ -2,6 +2,7 @@
 // element type only says how operands are stored.
 #include "api.h"
 #include "common.h"
+#include "draft_api.h"
 
 namespace {
 
@@ -173,7 +174,7 @@ add_residual_kernel(float *__restrict__ residual, const T *__restrict__ branch, 
 
 template <typename T>
 __global__ void __launch_bounds__(kBlock)
-rope_kv_store_kernel(T *__restrict__ qkv, const int32_t *__restrict__ row_pos, const int32_t *__restrict__ row_seg,
+rope_kv_store_kernel(T *__restrict__ qkv, const int32_t *__restrict__ row_pos, const int32_t *__restrict__ row_slot, const int32_t *__restrict__ row_seg,
                      const int32_t *__restrict__ tables, int table_stride, const float *__restrict__ cos_table,
                      const float *__restrict__ sin_table, T *__restrict__ k_pages, T *__restrict__ v_pages, int heads,
                      int kv_heads, int head_dim, int v_dim, int rope_dims, int pairing, int page_size, int key_chunk, int store_kv) {
@@ -199,8 +200,9 @@ rope_kv_store_kernel(T *__restrict__ qkv, const int32_t *__restrict__ row_pos, c
         // a layer that reads another layer's cache still rotates nothing else
         return;
     }
-    const int page = tables[(size_t)seg * table_stride + pos / page_size];
-    const int off = pos % page_size;
+    const int slot = row_slot ? row_slot[r] : pos;
+    const int page = tables[(size_t)seg * table_stride + slot / page_size];
+    const int off = slot % page_size;
     const T *krow = row + (size_t)heads * head_dim;
     const T *vrow = krow + (size_t)kv_heads * head_dim;
     // keys: rotated lanes, then the lanes rotary leaves alone
@@ -349,7 +351,7 @@ extern "C" int fllm_add_residual(float *residual, const void *branch, int rows, 
 // and every piece reads angles, 16 rows of 32 + 8 heads of 128 were 4.47 us instead of 4.23, of 64 + 8 with 64 lanes turning 5.44 instead of 5.00.
 template <int RB, int U>
 __global__ void __launch_bounds__(kBlock)
-rope_kv_store_vec_kernel(bf16_t *__restrict__ qkv, const int32_t *__restrict__ row_pos, const int32_t *__restrict__ row_seg,
+rope_kv_store_vec_kernel(bf16_t *__restrict__ qkv, const int32_t *__restrict__ row_pos, const int32_t *__restrict__ row_slot, const int32_t *__restrict__ row_seg,
                          const int32_t *__restrict__ tables, int table_stride, const float *__restrict__ cos_table,
                          const float *__restrict__ sin_table, bf16_t *__restrict__ k_pages, bf16_t *__restrict__ v_pages,
                          int rows, int heads, int kv_heads, int head_dim, int v_dim, int rope_dims, int page_size, int store_kv) {
@@ -364,23 +366,23 @@ rope_kv_store_vec_kernel(bf16_t *__restrict__ qkv, const int32_t *__restrict__ r
     __shared__ int s_pos[RB], s_page[RB], s_off[RB], s_run;
     if constexpr (RB == 1) {
         if (threadIdx.x == 0) {
-            const int seg = row_seg[r0], pos = row_pos[r0];
+            const int seg = row_seg[r0], pos = row_pos[r0], slot = row_slot ? row_slot[r0] : pos;
             s_pos[0] = seg < 0 ? -1 : pos;
-            s_page[0] = (store_kv && seg >= 0) ? tables[(size_t)seg * table_stride + pos / page_size] : 0;
-            s_off[0] = pos % page_size;
+            s_page[0] = (store_kv && seg >= 0) ? tables[(size_t)seg * table_stride + slot / page_size] : 0;
+            s_off[0] = slot % page_size;
             s_run = 0;
         }
     } else if ((int)threadIdx.x < kWave) {      // one wave: a lane a row, so that the rows are asked for together
         const int i = min((int)threadIdx.x, nrows - 1), r = r0 + i;
-        const int seg = row_seg[r], pos = row_pos[r];
-        const int seg0 = __builtin_amdgcn_readfirstlane(seg), pos0 = __builtin_amdgcn_readfirstlane(pos);
-        const bool follows = seg == seg0 && pos == pos0 + i;
-        const bool run = RB == 8 && store_kv && nrows == RB && seg0 >= 0 && (pos0 & (RB - 1)) == 0 && page_size % RB == 0 && __all(follows);
-        const int page = (store_kv && seg >= 0) ? tables[(size_t)seg * table_stride + pos / page_size] : 0;
+        const int seg = row_seg[r], pos = row_pos[r], slot = row_slot ? row_slot[r] : pos;
+        const int seg0 = __builtin_amdgcn_readfirstlane(seg), slot0 = __builtin_amdgcn_readfirstlane(slot);
+        const bool follows = seg == seg0 && slot == slot0 + i;
+        const bool run = RB == 8 && store_kv && nrows == RB && seg0 >= 0 && (slot0 & (RB - 1)) == 0 && page_size % RB == 0 && __all(follows);
+        const int page = (store_kv && seg >= 0) ? tables[(size_t)seg * table_stride + slot / page_size] : 0;
         if ((int)threadIdx.x < nrows) {
             s_pos[i] = seg < 0 ? -1 : pos;
             s_page[i] = page;
-            s_off[i] = pos % page_size;
+            s_off[i] = slot % page_size;
         }
         if (threadIdx.x == 0) s_run = run;
     }
@@ -467,11 +469,11 @@ rope_kv_store_vec_kernel(bf16_t *__restrict__ qkv, const int32_t *__restrict__ r
     }
 }
 
-extern "C" int fllm_rope_kv_store(void *qkv, const int32_t *row_pos, const int32_t *row_seg, const int32_t *tables,
-                                  int table_stride, const float *cos_table, const float *sin_table, int table_positions,
-                                  void *k_pages, void *v_pages, int num_pages, int rows, int heads, int kv_heads,
-                                  int head_dim, int v_dim, int rope_dims, int pairing, int page_size, int key_chunk, int dtype,
-                                  int store_kv, hipStream_t stream) {
+// row_slot null: a row's slot is its position
+extern "C" int fllm_rope_kv_store_at(void *qkv, const int32_t *row_pos, const int32_t *row_slot, const int32_t *row_seg, const int32_t *tables,
+                                     int table_stride, const float *cos_table, const float *sin_table, void *k_pages, void *v_pages, int num_pages,
+                                     int rows, int heads, int kv_heads, int head_dim, int v_dim, int rope_dims, int pairing, int page_size,
+                                     int key_chunk, int dtype, int store_kv, hipStream_t stream) {
     FLLM_REQUIRE(rows >= 0 && heads > 0 && kv_heads > 0 && head_dim > 0 && v_dim > 0 && page_size > 0 && table_stride > 0,
                  "rope_kv_store: bad sizes");
     FLLM_REQUIRE(rope_dims >= 0 && rope_dims <= head_dim && rope_dims % 2 == 0,
@@ -479,10 +481,9 @@ extern "C" int fllm_rope_kv_store(void *qkv, const int32_t *row_pos, const int32
     FLLM_REQUIRE(pairing == 0 || pairing == 1, "rope_kv_store: unknown pairing %d", pairing);
     FLLM_REQUIRE(!store_kv || (k_pages && v_pages && num_pages > 0), "rope_kv_store: pages missing");
     FLLM_REQUIRE(key_chunk > 0 && head_dim % key_chunk == 0, "rope_kv_store: keys of %d lanes cannot lie in chunks of %d", head_dim, key_chunk);
-    (void)table_positions;
     if (rows == 0) return 0;
     if (dtype == FLLM_F32)
-        hipLaunchKernelGGL(rope_kv_store_kernel<float>, dim3(rows), dim3(kBlock), 0, stream, (float *)qkv, row_pos, row_seg,
+        hipLaunchKernelGGL(rope_kv_store_kernel<float>, dim3(rows), dim3(kBlock), 0, stream, (float *)qkv, row_pos, row_slot, row_seg,
                            tables, table_stride, cos_table, sin_table, (float *)k_pages, (float *)v_pages, heads, kv_heads,
                            head_dim, v_dim, rope_dims, pairing, page_size, key_chunk, store_kv);
     else if (dtype == FLLM_BF16 && pairing == 1 && key_chunk == 8 && head_dim % 8 == 0 && v_dim % 8 == 0 && rope_dims % 8 == 0 && ((uintptr_t)qkv & 15) == 0 &&
@@ -495,23 +496,33 @@ extern "C" int fllm_rope_kv_store(void *qkv, const int32_t *row_pos, const int32
         const bool many = (long)(store_kv ? heads + kv_heads : heads) * (head_dim / 8) * 8 > 3 * 4 * kBlock;
         auto portion = [&](auto kernel) {
             hipLaunchKernelGGL(kernel, dim3((rows + 7) / 8, 4), dim3(kBlock), 0, stream, (bf16_t *)qkv, row_pos,
-                               row_seg, tables, table_stride, cos_table, sin_table, (bf16_t *)k_pages, (bf16_t *)v_pages, rows,
+                               row_slot, row_seg, tables, table_stride, cos_table, sin_table, (bf16_t *)k_pages, (bf16_t *)v_pages, rows,
                                heads, kv_heads, head_dim, v_dim, rope_dims, page_size, store_kv);
         };
         if (rows >= 256 && many) portion(rope_kv_store_vec_kernel<8, 4>);
         else if (rows >= 256) portion(rope_kv_store_vec_kernel<8, 1>);
         else
-            hipLaunchKernelGGL((rope_kv_store_vec_kernel<1, 1>), dim3(rows), dim3(kBlock), 0, stream, (bf16_t *)qkv, row_pos, row_seg,
+            hipLaunchKernelGGL((rope_kv_store_vec_kernel<1, 1>), dim3(rows), dim3(kBlock), 0, stream, (bf16_t *)qkv, row_pos, row_slot, row_seg,
                                tables, table_stride, cos_table, sin_table, (bf16_t *)k_pages, (bf16_t *)v_pages, rows, heads,
                                kv_heads, head_dim, v_dim, rope_dims, page_size, store_kv);
     }
     else if (dtype == FLLM_BF16)
         hipLaunchKernelGGL(rope_kv_store_kernel<bf16_t>, dim3(rows), dim3(kBlock), 0, stream, (bf16_t *)qkv, row_pos,
-                           row_seg, tables, table_stride, cos_table, sin_table, (bf16_t *)k_pages, (bf16_t *)v_pages, heads,
+                           row_slot, row_seg, tables, table_stride, cos_table, sin_table, (bf16_t *)k_pages, (bf16_t *)v_pages, heads,
                            kv_heads, head_dim, v_dim, rope_dims, pairing, page_size, key_chunk, store_kv);
     else
         FLLM_REQUIRE(false, "rope_kv_store: unknown dtype %d", dtype);
     return fllm_check_launch("rope_kv_store");
+}
+
+extern "C" int fllm_rope_kv_store(void *qkv, const int32_t *row_pos, const int32_t *row_seg, const int32_t *tables,
+                                  int table_stride, const float *cos_table, const float *sin_table, int table_positions,
+                                  void *k_pages, void *v_pages, int num_pages, int rows, int heads, int kv_heads,
+                                  int head_dim, int v_dim, int rope_dims, int pairing, int page_size, int key_chunk, int dtype,
+                                  int store_kv, hipStream_t stream) {
+    (void)table_positions;
+    return fllm_rope_kv_store_at(qkv, row_pos, nullptr, row_seg, tables, table_stride, cos_table, sin_table, k_pages, v_pages, num_pages, rows, heads,
+                                 kv_heads, head_dim, v_dim, rope_dims, pairing, page_size, key_chunk, dtype, store_kv, stream);
 }
 
 namespace {

@@ -54,6 +54,7 @@ _lib = None
 
 
 ABI_VERSION = 26
+DRAFT_ABI_VERSION = 1         # of csrc/draft_api.h
 
 
 def load_library(build_if_missing: bool = True):
@@ -76,6 +77,10 @@ def load_library(build_if_missing: bool = True):
     if lib.fllm_abi_version() != ABI_VERSION:
         raise KernelError(f"the HIP kernel library {path} has interface version {lib.fllm_abi_version()}, this package needs "
                           f"{ABI_VERSION}: build it again (python -m fllm_amd.kernels.build)")
+    lib.fllm_draft_abi_version.restype = c_int
+    if lib.fllm_draft_abi_version() != DRAFT_ABI_VERSION:
+        raise KernelError(f"the HIP kernel library {path} has version {lib.fllm_draft_abi_version()} of the drafts' interface, this package "
+                          f"needs {DRAFT_ABI_VERSION}: build it again (python -m fllm_amd.kernels.build)")
     sig = {
         "fllm_embed": [c_void, c_void, c_void, c_int, c_int, c_int, c_int, c_float, c_void],
         "fllm_rmsnorm": [c_void, c_void, c_void, c_void, c_int, c_int, c_float, c_int, c_void],
@@ -199,6 +204,14 @@ def load_library(build_if_missing: bool = True):
         "fllm_experts_grouped_ungated": [c_void, c_int, c_void, c_int, c_int, c_void, c_void, c_int, c_int, c_int, c_int, c_void, c_void,
                                          c_void, c_void, c_void],
         "fllm_experts_up": [c_void, c_int, c_void, c_int, c_int, c_void, c_int, c_int, c_int, c_void, c_int, c_void],
+        "fllm_tree_attention": [c_void, c_int, c_void, c_void, c_void, c_int, c_void, c_void, c_int, c_void, c_void, c_int, c_void, c_int, c_int,
+                                c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_void, c_int, c_int, c_int, c_void],
+        "fllm_follow_tree": [c_void, c_void, c_void, c_int, c_void, c_int, c_void, c_int, c_void, c_void, c_void],
+        "fllm_move_tokens": [c_void, c_void, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_void, c_int, c_int, c_void, c_void, c_int,
+                             c_void, c_void],
+        "fllm_copy_pages": [c_void, c_void, c_void, c_void, c_int, c_void, c_void, c_int, c_void],
+        "fllm_rope_kv_store_at": [c_void, c_void, c_void, c_void, c_void, c_int, c_void, c_void, c_void, c_void, c_int, c_int, c_int, c_int,
+                                  c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_void],
     }
     for name, args in sig.items():
         fn = getattr(lib, name)
@@ -259,6 +272,37 @@ def _dense(t: torch.Tensor, name: str, dtype=None, shape=None) -> None:
         raise KernelError(f"{name} must be {dtype}, is {t.dtype}")
     if shape is not None and t.shape != tuple(shape):      # a torch.Size is a tuple
         raise KernelError(f"{name} must have shape {tuple(shape)}, has {tuple(t.shape)}")
+
+
+def _here(t: torch.Tensor, name: str, device: int) -> None:
+    if not t.is_cuda:
+        raise KernelError(f"{name} must be on the GPU")
+    if t.device.index != device:
+        raise KernelError(f"{name} is on device {t.device.index}, the current device is {device}")
+
+
+def _held(t: torch.Tensor, name: str, device: int, dtype, shape) -> None:
+    """As `_dense`, and on the current device."""
+    if t.device.index != device or t.dtype != dtype or t.shape != shape or not t.is_contiguous():
+        _dense(t, name, dtype, shape)
+        _here(t, name, device)
+
+
+def tree_rows(parents: Sequence[int], words: Optional[int] = None) -> Tuple[list, list]:
+    """(depths, seen) of one tree of drafted tokens: for every node how many nodes lie above it, and as `words` signed 64-bit numbers (by
+    default as many as the nodes need) the bits of its ancestors and itself, a row of `Ops.tree_attention`'s `seen`.  Node 0 is the
+    root; parents[0] does not count."""
+    words = max(1, -(-len(parents) // 64)) if words is None else int(words)
+    if len(parents) > 64 * words:
+        raise ValueError(f"{len(parents)} nodes need more than {words} words")
+    depths, bits = [], []
+    for i, parent in enumerate(parents):
+        if i > 0 and not 0 <= parent < i:
+            raise ValueError(f"node {i} has parent {parent}: a parent has a lower number")
+        depths.append(depths[parent] + 1 if i else 0)
+        bits.append((bits[parent] if i else 0) | 1 << i)
+    signed = lambda w: w - (1 << 64) if w >> 63 else w
+    return depths, [[signed(b >> 64 * w & (1 << 64) - 1) for w in range(words)] for b in bits]
 
 
 @functools.lru_cache(maxsize=256)
@@ -430,6 +474,10 @@ class Ops:
             return device, raw(device)
         stream = torch.cuda.current_stream()
         return stream.device_index, stream.cuda_stream
+
+    @staticmethod
+    def _current_device() -> int:
+        return Ops._current_stream()[0]
 
     @staticmethod
     def _stream() -> int:
@@ -849,9 +897,11 @@ class Ops:
     def rope_kv_store(self, qkv: torch.Tensor, row_pos: torch.Tensor, row_seg: torch.Tensor, tables: torch.Tensor,
                       cos: torch.Tensor, sin: torch.Tensor, k_pages: Optional[torch.Tensor],
                       v_pages: Optional[torch.Tensor], heads: int, kv_heads: int, head_dim: int, rope_dims: int,
-                      pairing: int, page_size: int, v_dim: Optional[int] = None, key_chunk: int = 8) -> None:
+                      pairing: int, page_size: int, v_dim: Optional[int] = None, key_chunk: int = 8,
+                      row_slot: Optional[torch.Tensor] = None) -> None:
         """`v_dim`: lanes of a value head where they differ from the keys'; `key_chunk`: values of a key that lie together
-        in a page (8; 1 for head sizes that are no multiple of 8)."""
+        in a page (8; 1 for head sizes that are no multiple of 8); `row_slot` (int32 [rows]): the slots of the request's cache
+        that the rows are stored in, where those are not their positions (the nodes of a tree of drafted tokens)."""
         rows = qkv.shape[0]
         v_dim = head_dim if v_dim is None else int(v_dim)
         _dense(qkv, "qkv", None, (rows, (heads + kv_heads) * head_dim + kv_heads * v_dim))
@@ -871,6 +921,13 @@ class Ops:
             num_pages = k_pages.shape[0]
             _dense(k_pages, "k_pages", qkv.dtype, (num_pages, kv_heads, head_dim // key_chunk, page_size, key_chunk))
             _dense(v_pages, "v_pages", qkv.dtype, (num_pages, kv_heads, v_dim, page_size))
+        if row_slot is not None:
+            _dense(row_slot, "row_slot", torch.int32, (rows,))
+            self._check(self.lib.fllm_rope_kv_store_at(
+                _ptr(qkv), _ptr(row_pos), _ptr(row_slot), _ptr(row_seg), _ptr(tables), tables.shape[1], _ptr(cos), _ptr(sin), _ptr(k_pages),
+                _ptr(v_pages), num_pages, rows, heads, kv_heads, head_dim, v_dim, rope_dims, pairing, page_size, key_chunk,
+                _DTYPE_CODE[qkv.dtype], 1 if store else 0, self._stream()))
+            return
         self._check(self.lib.fllm_rope_kv_store(
             _ptr(qkv), _ptr(row_pos), _ptr(row_seg), _ptr(tables), tables.shape[1], _ptr(cos), _ptr(sin), cos.shape[0],
             _ptr(k_pages), _ptr(v_pages), num_pages, rows, heads, kv_heads, head_dim, v_dim, rope_dims, pairing, page_size,
@@ -1981,6 +2038,136 @@ class Ops:
             int(chunk), int(window), int(keep_first), _ptr(talk), _ptr(spread), key_chunk, _DTYPE_CODE[q.dtype], int(max_context),
             self._stream()))
         return out
+
+    # ---- trees of drafted tokens --------------------------------------------------------------------------------------------
+    # A request has `kept` tokens in its pages; a draft adds rows, the nodes of a tree of candidate continuations.  Segment s has the rows
+    # seg_start[s] .. seg_start[s + 1] - 1, its nodes 0, 1, ..: node i lies in slot kept[s] + i of the request's cache, node 0 is the
+    # request's newest token, and every other node's parent has a lower number.  A step on a tree is rope_kv_store(row_slot=) and
+    # tree_attention in every layer, the choice of a token at every node (sample, argmax), follow_tree and move_tokens.
+    def tree_attention(self, q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Tensor, row_pos: torch.Tensor,
+                       seg_start: torch.Tensor, kept: torch.Tensor, seen: torch.Tensor, out: torch.Tensor, heads: int, kv_heads: int,
+                       head_dim: int, page_size: int, scale: float, max_context: int, window: Optional[int] = None,
+                       sinks: Optional[torch.Tensor] = None, v_dim: Optional[int] = None, key_chunk: int = 8,
+                       max_nodes: Optional[int] = None) -> torch.Tensor:
+        """Softmax attention of the nodes: row r of segment s sees the `kept[s]` tokens of its request and the nodes of its segment whose
+        bits are set in `seen[r]` (int64 [rows, words], bit j % 64 of word j / 64: node j, for a tree its ancestors and itself;
+        `tree_rows` makes them); with a `window`, of both only what lies at positions above row_pos[r] - window (a kept token at its
+        slot, a node at its `row_pos`).  `sinks` (float32 [heads]): exp(sinks[head]) joins the denominator.  A row that sees nothing
+        gives zeros; rows ahead of the first segment or behind the last are left as they are.  What a row does not see does not reach
+        it, whatever the slots hold; a table entry that names no page is not seen.
+        `q` may be a column slice of a wider matrix; `v_dim`, `key_chunk` as in `attention`; `out` has memory of its own.
+        `max_context` bounds kept + nodes over the segments, `max_nodes` (64 * words where it is not given) the nodes: a segment's rows
+        beyond it are left as they are."""
+        rows = q.shape[0]
+        v_dim = head_dim if v_dim is None else int(v_dim)
+        device = self._current_device()
+        _need(q.is_cuda and q.dim() == 2 and q.stride(1) == 1 and q.shape[1] == heads * head_dim,
+              f"q must be [rows, {heads * head_dim}] with unit column stride")
+        dtype = q.dtype
+        _need(dtype in _DTYPE_CODE, f"dtype {dtype} unsupported")
+        _need(key_chunk > 0 and head_dim % key_chunk == 0, "tree_attention: bad chunk of key values")
+        _here(q, "q", device)
+        num_pages = k_pages.shape[0]
+        _held(k_pages, "k_pages", device, dtype, (num_pages, kv_heads, head_dim // key_chunk, page_size, key_chunk))
+        _held(v_pages, "v_pages", device, dtype, (num_pages, kv_heads, v_dim, page_size))
+        _need(tables.dim() == 2, "tables must be [segments, pages]")
+        segs, stride = tables.shape
+        _held(tables, "tables", device, torch.int32, (segs, stride))
+        _held(row_pos, "row_pos", device, torch.int32, (rows,))
+        _held(seg_start, "seg_start", device, torch.int32, (segs + 1,))
+        _held(kept, "kept", device, torch.int32, (segs,))
+        _need(seen.dim() == 2 and seen.shape[1] > 0, "seen must be [rows, words]")
+        words = seen.shape[1]
+        _held(seen, "seen", device, torch.int64, (rows, words))
+        _held(out, "out", device, dtype, (rows, heads * v_dim))
+        if sinks is not None:
+            _held(sinks, "sinks", device, torch.float32, (heads,))
+        most = 64 * words if max_nodes is None else int(max_nodes)
+        _need(0 <= most <= 64 * words, f"max_nodes {most}: {words} words hold the bits of at most {64 * words}")
+        self._check(self.lib.fllm_tree_attention(
+            _ptr(q), q.stride(0) if rows > 1 else heads * head_dim, _ptr(k_pages), _ptr(v_pages), _ptr(tables), stride, _ptr(row_pos),
+            _ptr(seg_start), segs, _ptr(kept), _ptr(seen), words, _ptr(out), rows, heads, kv_heads, head_dim, v_dim, page_size, num_pages,
+            float(scale), int(window) if window else 0, key_chunk, _ptr(sinks), _DTYPE_CODE[dtype], min(most, rows), int(max_context),
+            self._stream()))
+        return out
+
+    def follow_tree(self, drafted: torch.Tensor, parents: torch.Tensor, seg_start: torch.Tensor, chosen: torch.Tensor, path: torch.Tensor,
+                    length: torch.Tensor, newest: torch.Tensor) -> None:
+        """Which drafted tokens the model chose itself.  `drafted` (the nodes' tokens), `parents` (node numbers, lower than the node's own;
+        the root's does not count) and `chosen` (the token that the model chose behind every node) are int32 [rows].  From node 0 on
+        the walk goes to the lowest child whose token is what was chosen at its parent.  `path` (int32 [segments, n], n the most nodes
+        wanted): its nodes, -1 behind them; `length`: how many; `newest`: what was chosen at the last, the request's next token.  A
+        segment without rows: length 0, newest -1."""
+        rows, segs = drafted.shape[0], seg_start.shape[0] - 1
+        device = self._current_device()
+        _need(drafted.dim() == 1 and seg_start.dim() == 1 and segs >= 0, "drafted must be [rows], seg_start [segments + 1]")
+        _held(drafted, "drafted", device, torch.int32, (rows,))
+        _held(parents, "parents", device, torch.int32, (rows,))
+        _held(chosen, "chosen", device, torch.int32, (rows,))
+        _held(seg_start, "seg_start", device, torch.int32, (segs + 1,))
+        _need(path.dim() == 2 and path.shape[1] > 0, "path must be [segments, nodes]")
+        most = path.shape[1]
+        _held(path, "path", device, torch.int32, (segs, most))
+        _held(length, "length", device, torch.int32, (segs,))
+        _held(newest, "newest", device, torch.int32, (segs,))
+        self._check(self.lib.fllm_follow_tree(_ptr(drafted), _ptr(parents), _ptr(seg_start), segs, _ptr(chosen), rows, _ptr(path), most,
+                                              _ptr(length), _ptr(newest), self._stream()))
+
+    def move_tokens(self, k_store: torch.Tensor, v_store: Optional[torch.Tensor], tables: torch.Tensor, kept: torch.Tensor, path: torch.Tensor,
+                    length: torch.Tensor) -> None:
+        """Keys and values move up inside their requests' pages, in every layer: slot kept[s] + path[s, i] to slot kept[s] + i, for
+        i < length[s] (what `follow_tree` leaves).  A path rises; it ends ahead of an entry that does not, or is negative.
+        `k_store` [layers, pages, kv_heads, k_dim / chunk, page_size, chunk] (or [layers, pages, kv_heads, page_size, k_dim]) and
+        `v_store` [layers, pages, kv_heads, v_dim, page_size] (None where keys are all there is): the pages of all layers that share the
+        block tables `tables` [segments, pages].  Slots without a page are left out."""
+        device = self._current_device()
+        _need(k_store.dim() in (5, 6), "k_store must be [layers, pages, kv_heads, k_dim / chunk, page_size, chunk]")
+        layers, pages, kv_heads = k_store.shape[:3]
+        page_size, chunk = k_store.shape[-2:]
+        k_dim = chunk * (k_store.shape[3] if k_store.dim() == 6 else 1)
+        _need(k_store.dtype in _DTYPE_CODE, f"dtype {k_store.dtype} unsupported")
+        _held(k_store, "k_store", device, k_store.dtype, k_store.shape)
+        v_dim = 0
+        if v_store is not None:
+            _need(v_store.dim() == 5, "v_store must be [layers, pages, kv_heads, v_dim, page_size]")
+            v_dim = v_store.shape[3]
+            _held(v_store, "v_store", device, k_store.dtype, (layers, pages, kv_heads, v_dim, page_size))
+        _need(tables.dim() == 2, "tables must be [segments, pages]")
+        segs, stride = tables.shape
+        _held(tables, "tables", device, torch.int32, (segs, stride))
+        _held(kept, "kept", device, torch.int32, (segs,))
+        _need(path.dim() == 2 and path.shape[1] > 0, "path must be [segments, nodes]")
+        _held(path, "path", device, torch.int32, (segs, path.shape[1]))
+        _held(length, "length", device, torch.int32, (segs,))
+        self._check(self.lib.fllm_move_tokens(
+            _ptr(k_store), _ptr(v_store), layers, pages, kv_heads, k_dim, v_dim, page_size, chunk, k_store.element_size(), _ptr(tables), stride,
+            segs, _ptr(kept), _ptr(path), path.shape[1], _ptr(length), self._stream()))
+
+    def copy_pages(self, stores: Sequence[torch.Tensor], source: Sequence[int], target: Sequence[int]) -> None:
+        """Page source[i] is copied to page target[i] in every layer of every store ([layers, pages, ...], at most 8 of them): what a request
+        takes over of another's when it goes on from the same tokens (`CacheManager.fork_request` names the pages), or a cache that is
+        packed.  No page is a target twice, or a source and a target."""
+        device = self._current_device()
+        pairs = len(source)
+        _need(len(target) == pairs, f"{pairs} pages to copy from, {len(target)} to copy to")
+        _need(0 < len(stores) <= 8, f"{len(stores)} stores: 1 to 8 are copied at a time")
+        targets = set(target)
+        _need(len(targets) == pairs, "a page is copied to twice")
+        _need(targets.isdisjoint(source), "a page is copied from and to")
+        sizes = []
+        for n, store in enumerate(stores):
+            _need(store.dim() >= 2, f"store {n} must be [layers, pages, ...]")
+            _held(store, f"store {n}", device, store.dtype, store.shape)
+            pages = store.shape[1]
+            _need(pairs == 0 or (0 <= min(source) and max(source) < pages and 0 <= min(target) and max(target) < pages),
+                  f"store {n} has {pages} pages")
+            sizes.append((store.shape[0], pages, store[0, 0].numel() * store.element_size() if pages and store.shape[0] else 0))
+        if pairs == 0:
+            return
+        counts = [(ctypes.c_int64 * len(stores))(*column) for column in zip(*sizes)]
+        numbers = ctypes.c_int32 * pairs
+        self._check(self.lib.fllm_copy_pages((ctypes.c_void_p * len(stores))(*[_ptr(t) for t in stores]), *counts, len(stores), numbers(*source),
+                                             numbers(*target), pairs, self._stream()))
 
     # ---- attention over cached latents ------------------------------------------------------------------------------------
     def latent_rope_store(self, joint: torch.Tensor, dkv_at: int, rank: int, rot: int, c_weight: torch.Tensor, eps: float, heads: int, dim: int,
