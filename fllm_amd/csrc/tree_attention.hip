@@ -6,6 +6,9 @@
 #include "draft_api.h"
 #include "tree_attention.h"
 
+int fllm_tree_attention_fast(const TreeArgs &a, int head_dim, int v_dim, int key_chunk, int dtype, int max_context,
+                             hipStream_t stream);      // tree_attention_mfma.hip; 1: shape declined
+
 namespace {
 
 constexpr int kBlock = 256;
@@ -32,7 +35,7 @@ tree_attention_generic_kernel(TreeArgs p, int head_dim, int v_dim, int key_chunk
     if (r - row0 >= p.max_nodes) return;
     const int kept = max(p.kept[seg], 0);
     const long slots = (long)p.table_stride * p.page_size;
-    const int n = (int)min((long)kept + nodes, slots);
+    const int n = (int)min((long)kept + nodes, min(slots, (long)INT_MAX - 4096));
     const int pos = p.row_pos[r];
     const int lo = p.window > 0 ? pos - p.window + 1 : INT_MIN;      // the first position that the row sees
     const int kvh = h / (p.heads / p.kv_heads);
@@ -92,7 +95,7 @@ tree_attention_generic_kernel(TreeArgs p, int head_dim, int v_dim, int key_chunk
         const float sink = p.sinks[h];
         const float m_all = fmaxf(m, sink);
         keep = m == -INFINITY ? 0.f : expf(m - m_all);
-        l = l * keep + (sink == -INFINITY ? 0.f : expf(sink - m_all));
+        l = l * keep + (sink == m_all ? 1.f : expf(sink - m_all));
     }
     const float inv = l == 0.f ? 0.f : keep / l;      // a NaN stays one
 #pragma unroll
@@ -145,6 +148,8 @@ extern "C" int fllm_tree_attention(const void *q, int q_stride, const void *k_pa
     a.window = window;
     a.max_nodes = max_nodes;
     a.scale = scale;
+    const int fast = fllm_tree_attention_fast(a, head_dim, v_dim, key_chunk, dtype, max_context, stream);
+    if (fast <= 0) return fast;
     const dim3 grid(rows, heads);
     const size_t smem = (size_t)(head_dim + kBlock + kWaves) * sizeof(float);
     if (dtype == FLLM_F32)
