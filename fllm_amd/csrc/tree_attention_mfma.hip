@@ -12,49 +12,26 @@
 //             the slots 4 g + i: the operands are the elements of 16-byte loads, and the scores are the second product's operand as they are.
 // Slots that every row of the tile sees need no mask; a block that holds nodes, the end, the window's edge or a page that is none gets a
 // 64-bit mask a row.
-#include <algorithm>
 #include "common.h"
 #include "draft_api.h"
 #include "tree_attention.h"
 
+int fllm_tree_attention_wide(const TreeArgs &a, int max_context, hipStream_t stream);      // tree_attention_wide.hip
+
 namespace {
 
-constexpr int kWaves = 4;
-constexpr int kThreads = kWaves * kWave;
-constexpr float kLog2e = 1.4426950408889634f;
-typedef __attribute__((ext_vector_type(2))) float f32x2_t;
-
-// What a launch adds to TreeArgs: how the slots are split and where the parts of a tile meet.
-struct TreeSplit {
-    int tiles;            // row tiles a request at most
-    int splits, per;      // parts of the slots, slots a part (the last takes what is left)
-    int *counters;        // one per (request, key/value head, tile), zero between launches
-    float *parts;         // [request, key/value head, tile][split][16 NT rows of D outputs, then of a maximum and a sum]
-    float scale;          // >= 0: the sign has gone into the queries
-    int negate;
-};
 
 template <typename T> struct Operand;
 template <> struct Operand<bf16_t> {
     typedef bf16x8_t vec;
-    static constexpr int kTiles = 4;      // score tiles of 16 slots a block
+    static constexpr int kStep = 32;      // slots that a value load of all lanes covers
     static constexpr int kPer = 8;        // elements of a 16-byte load
 };
 template <> struct Operand<float> {
     typedef f32x4_t vec;
-    static constexpr int kTiles = 2;
+    static constexpr int kStep = 16;
     static constexpr int kPer = 4;
 };
-
-__device__ __forceinline__ bf16x8_t pack8(const f32x4_t &lo, const f32x4_t &hi) {
-    bf16x8_t p;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        p[i] = (bf16_t)lo[i];
-        p[4 + i] = (bf16_t)hi[i];
-    }
-    return p;
-}
 
 // from slots 16 j + 4 g + i of two tiles j to slots 8 g .. 8 g + 7
 __device__ __forceinline__ bf16x8_t neighbours(bf16x8_t p) {
@@ -69,40 +46,46 @@ __device__ __forceinline__ bf16x8_t neighbours(bf16x8_t p) {
     return __builtin_bit_cast(bf16x8_t, w);
 }
 
-__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
-
-// the `count` lowest bits
-__device__ __forceinline__ unsigned long long low_bits(int count) {
-    return count <= 0 ? 0ull : count >= 64 ? ~0ull : (1ull << count) - 1;
-}
-
 constexpr int q_pitch(int D, bool wide) { return D + (wide ? 4 : 8); }      // elements of a query row in LDS
 
-template <typename T, int D, int NT>
+// The waves are RG groups of rows times KW groups of slots.  Outputs of all slots' groups lie in LDS at a time, or those of half of them, which
+// the other half then adds to its own.
+template <int D, int ROWS, int KW>
+constexpr int groups_together() {
+    return (size_t)KW * ROWS * (D + 4) * sizeof(float) > 140 * 1024 ? KW / 2 : KW;
+}
+template <typename T, int D, int ROWS, int KW>
+constexpr size_t lds_area() {      // the queries while there are slots, the outputs afterwards
+    const size_t queries = (size_t)ROWS * q_pitch(D, sizeof(T) == 4) * sizeof(T), outputs = (size_t)groups_together<D, ROWS, KW>() * ROWS * (D + 4) * sizeof(float);
+    return queries > outputs ? queries : outputs;
+}
+template <typename T, int D, int ROWS, int KW>
 constexpr size_t lds_bytes() {
-    return (size_t)16 * NT * q_pitch(D, sizeof(T) == 4) * sizeof(T) + (size_t)kWaves * 16 * NT * (D + 4 + 2) * sizeof(float);
+    return lds_area<T, D, ROWS, KW>() + (size_t)KW * ROWS * 2 * sizeof(float);
 }
 
+// H: value loads of all lanes a block, 32 slots (float32: 16) each.
 // PSH: pages of 1 << PSH tokens; of 8, two a score tile, otherwise of 16, 32 or 64.
-template <typename T, int D, int NT, int PSH, int EU>
-__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(EU, EU)))
+template <typename T, int D, int NT, int PSH, int H, int RG, int KW, int EU>
+__global__ void __launch_bounds__(RG * KW * kWave) __attribute__((amdgpu_waves_per_eu(EU, EU)))
 tree_attention_kernel(TreeArgs p, TreeSplit sp) {
     typedef typename Operand<T>::vec vec;
     constexpr bool kHalf = sizeof(T) == 2;
-    constexpr int TILES = Operand<T>::kTiles, PER = Operand<T>::kPer, KB = 16 * TILES;
+    constexpr int PER = Operand<T>::kPer, KB = Operand<T>::kStep * H, TILES = KB / 16, THREADS = RG * KW * kWave;
     constexpr int KD = D / (4 * PER);       // 16-byte loads of a key a lane
     constexpr bool P8 = PSH == 3;
     constexpr int PS = 1 << PSH, PMASK = PS - 1;
-    constexpr int DT = D / 16, NP = P8 ? 2 * TILES : TILES, ROWS = 16 * NT, QP = q_pitch(D, !kHalf), OP = D + 4;
+    constexpr int DT = D / 16, NP = P8 ? 2 * TILES : TILES, ROWS = 16 * NT * RG, WT = groups_together<D, ROWS, KW>(), QP = q_pitch(D, !kHalf), OP = D + 4;
     typedef const __attribute__((address_space(4))) int32_t *constant_t;      // the same for every lane: a scalar load
     // what a full exponent adds up to, in the halves of a word or in all of it
     constexpr unsigned kExponents = kHalf ? 0x7f807f80u : 0x7f800000u, kExponentStep = kHalf ? 0x00800080u : 0x00800000u,
                        kSigns = kHalf ? 0x80008000u : 0x80000000u;
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+    __shared__ int s_row[ROWS], s_lo[ROWS];      // a row's number (-1: none) and the first position it sees
     __shared__ int s_odd;      // a block held values that are not finite and had to be cleared
     T *qs = (T *)lds;                                                     // [ROWS][QP]
-    float *sm_o = (float *)(lds + (size_t)ROWS * QP * sizeof(T));         // [kWaves][ROWS][OP]
-    float *sm_m = sm_o + kWaves * ROWS * OP, *sm_l = sm_m + kWaves * ROWS;
+    float *sm_o = (float *)lds;                                           // [WT][ROWS][OP], when the queries have served
+    float *sm_m = (float *)(lds + lds_area<T, D, ROWS, KW>()), *sm_l = sm_m + KW * ROWS;
 
     // One grid dimension: the tiles of one (request, part, key/value head) lie on one die, one after the other, so that what the first
     // reads from memory the others find in its L2.
@@ -120,28 +103,19 @@ tree_attention_kernel(TreeArgs p, TreeSplit sp) {
     const int kept = min(kept0, n);
     const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int c = lane & 15, g = lane >> 4;
+    const int kw = wave / RG, at_row = wave % RG * (16 * NT) + c;      // the wave's slots, and the lane's row of its first tile
 
-    // the first position that a row sees, the lowest and highest over the tile
-    int lo_row[NT], lo_min = INT_MIN, lo_max = INT_MIN;
+    // the first position that a row sees, the lowest and highest over the tile (a node a lane)
+    int lo_min = INT_MIN, lo_max = INT_MIN;
     if (p.window > 0) {
-        lo_min = INT_MAX;
+        lo_min = lo_max = p.row_pos[row0 + first_node + min(lane, ntok - 1)] - p.window + 1;
 #pragma unroll
-        for (int t = 0; t < NT; t++) {
-            const int tq = (t * 16 + c) / G;
-            lo_row[t] = p.row_pos[row0 + first_node + min(tq, ntok - 1)] - p.window + 1;
-            lo_min = min(lo_min, lo_row[t]);
-            lo_max = max(lo_max, lo_row[t]);
-        }
-#pragma unroll
-        for (int step = 8; step > 0; step >>= 1) {
+        for (int step = 32; step > 0; step >>= 1) {
             lo_min = min(lo_min, __shfl_xor(lo_min, step));
             lo_max = max(lo_max, __shfl_xor(lo_max, step));
         }
         lo_min = __builtin_amdgcn_readfirstlane(lo_min);
         lo_max = __builtin_amdgcn_readfirstlane(lo_max);
-    } else {
-#pragma unroll
-        for (int t = 0; t < NT; t++) lo_row[t] = INT_MIN;
     }
     const int first = max(0, min(lo_min, kept)) / KB * KB;
     const int live = max(1, (int)min((long)sp.splits, ((long)n - first + sp.per - 1) / sp.per));      // parts that hold slots
@@ -166,25 +140,26 @@ tree_attention_kernel(TreeArgs p, TreeSplit sp) {
         }
         return pg;
     };
-    vec kf[TILES][KD], vf[2][DT];
+    vec kf[TILES][KD], vf[H][DT];
     // A lane's place in a page is the same in every block; the rest of an address is a scalar wherever one page serves all lanes.
     constexpr size_t kHeadBytes = (size_t)D * PS * sizeof(T);
     const unsigned k_lane = kHalf ? (unsigned)(g * PS + (P8 ? c & 7 : c)) * 16 : (unsigned)((g >> 1) * PS + (P8 ? c & 7 : c)) * 32 + (g & 1) * 16;
-    auto load_keys = [&](int kb, const Pages &pg) {
+    // piece j of a block's keys
+    auto load_keys = [&](int kb, const Pages &pg, int j) __attribute__((always_inline)) {
 #pragma unroll
         for (int t = 0; t < TILES; t++) {
             const char *base = (const char *)p.kp + (size_t)kvh * kHeadBytes + (P8 ? 0 : (size_t)((kb + 16 * t) & PMASK) * (8 * sizeof(T)));
             if (P8) base += (size_t)(c < 8 ? pg.page[P8 ? 2 * t : t] : pg.page[P8 ? 2 * t + 1 : t]) * nkv * kHeadBytes;
             else base += (size_t)pg.page[t] * nkv * kHeadBytes;
-#pragma unroll
-            for (int j = 0; j < KD; j++) kf[t][j] = __builtin_nontemporal_load((const vec *)(base + j * 64 * PS + k_lane));
+            kf[t][j] = __builtin_nontemporal_load((const vec *)(base + j * 64 * PS + k_lane));
         }
     };
     // values: bfloat16 the slots 32 h + 8 g .. + 7, float32 16 h + 4 g .. + 3
     const unsigned v_lane = (unsigned)(c * PS + (kHalf ? (P8 ? 0 : PSH == 4 ? 8 * (g & 1) : 8 * g) : (P8 ? 4 * (g & 1) : 4 * g))) * (unsigned)sizeof(T);
-    auto load_values = [&](int kb, const Pages &pg) {
+    // lanes 16 dt .. 16 dt + 15 of a block's values
+    auto load_values = [&](int kb, const Pages &pg, int dt) __attribute__((always_inline)) {
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
+        for (int h = 0; h < H; h++) {
             const char *base = (const char *)p.vp + (size_t)kvh * kHeadBytes;
             const size_t page_bytes = (size_t)nkv * kHeadBytes;
             if constexpr (kHalf) {
@@ -195,63 +170,77 @@ tree_attention_kernel(TreeArgs p, TreeSplit sp) {
                 if constexpr (P8) base += (size_t)(g < 2 ? pg.page[2 * h] : pg.page[2 * h + 1]) * page_bytes;
                 else base += (size_t)pg.page[h] * page_bytes + (size_t)((kb + 16 * h) & PMASK) * sizeof(T);
             }
-#pragma unroll
-            for (int dt = 0; dt < DT; dt++) vf[h][dt] = *(const vec *)(base + dt * 16 * PS * (int)sizeof(T) + v_lane);
+            vf[h][dt] = *(const vec *)(base + dt * 16 * PS * (int)sizeof(T) + v_lane);
         }
     };
-    // Which of the block's slots the lane's row of tile t sees, a bit a slot.
-    auto sight = [&](int t, int kb, unsigned bad) -> unsigned long long {
-        const int tq = (t * 16 + c) / G;
-        const int to_kept = kept - kb;
+    // The words of a block's nodes for the lane's row of tile t: the one that holds the first (bit j0 % 64) and the one behind it.
+    struct Words {
+        unsigned long long low, high;
+    };
+    auto words_of = [&](int t, int kb) {
+        const int w = max(kb - kept, 0) >> 6;
+        const int64_t *mine = p.seen + (size_t)max(s_row[at_row + t * 16], 0) * p.words;
+        return Words{(unsigned long long)mine[min(w, p.words - 1)], (unsigned long long)mine[min(w + 1, p.words - 1)]};
+    };
+    // Which of the block's slots the lane's row of tile t sees, a bit a slot; `at` is the position of node kb - kept + lane.
+    auto sight = [&](int t, int kb, unsigned bad, const Words &words, int at) -> unsigned long long {
+        const int to_kept = kept - kb, lo = s_lo[at_row + t * 16];
         unsigned long long bits = low_bits(to_kept);
-        if (p.window > 0) bits &= ~low_bits(lo_row[t] <= kb ? 0 : min(lo_row[t] - kb, 64));
+        if (p.window > 0) bits &= ~low_bits(lo <= kb ? 0 : min(lo - kb, 64));
         if (kb + KB > kept) {
             const int j0 = kb - kept;       // the node at the block's first slot
-            const int64_t *mine = p.seen + (size_t)(row0 + first_node + min(tq, ntok - 1)) * p.words;
             unsigned long long tree;
             if (j0 <= 0) {
-                tree = (unsigned long long)mine[0] << -j0;       // -j0 < KB
+                tree = words.low << -j0;       // -j0 < KB
             } else {
                 const int w = j0 >> 6, s = j0 & 63;
-                tree = w < p.words ? (unsigned long long)mine[w] >> s : 0ull;
-                if (s > 0 && w + 1 < p.words) tree |= (unsigned long long)mine[w + 1] << (64 - s);
+                tree = w < p.words ? words.low >> s : 0ull;
+                if (s > 0 && w + 1 < p.words) tree |= words.high << (64 - s);
             }
             if (p.window > 0) {      // a node's position, one a lane, against every row's edge
-                const int j = j0 + lane;
-                const int at = j >= 0 && j < nodes && lane < KB ? p.row_pos[row0 + j] : INT_MIN;
                 unsigned long long near = 0;
 #pragma unroll
                 for (int r = 0; r < 16; r++) {
-                    const unsigned long long one = __ballot(at >= __builtin_amdgcn_readlane(lo_row[t], r));
+                    const unsigned long long one = __ballot(at >= __builtin_amdgcn_readlane(lo, r));
                     near = c == r ? one : near;
                 }
                 tree &= near;
             }
             bits |= tree & ~low_bits(to_kept) & low_bits(n - kb);
         }
+        if (bad != 0) {
 #pragma unroll
-        for (int i = 0; i < NP; i++)
-            if (bad >> i & 1) bits &= ~(low_bits(P8 ? 8 : 16) << (i * (P8 ? 8 : 16)));
-        return tq < ntok ? bits : 0ull;
+            for (int i = 0; i < NP; i++)
+                if (bad >> i & 1) bits &= ~(low_bits(P8 ? 8 : 16) << (i * (P8 ? 8 : 16)));
+        }
+        return s_row[at_row + t * 16] < 0 ? 0ull : bits;
     };
 
     f32x4_t o[NT][DT];
     float m_run[NT], l_run[NT];      // the reference point in raw units; the sum over the lane's own slots
 #pragma unroll
     for (int t = 0; t < NT; t++) {
-        m_run[t] = -INFINITY;
+        m_run[t] = kNothing;
         l_run[t] = 0.f;
 #pragma unroll
         for (int dt = 0; dt < DT; dt++) o[t][dt] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
     }
     const float sc = sp.scale, tau = 8.0f / sc;
 
-    int kb = begin + wave * KB;
+    int kb = begin + kw * KB;
     Pages pg = block_pages(kb);
-    if (kb < end) load_keys(kb, pg);
+    if (kb < end) {
+#pragma unroll
+        for (int j = 0; j < KD; j++) load_keys(kb, pg, j);
+    }
     if (threadIdx.x == 0) s_odd = 0;
+    if ((int)threadIdx.x < ROWS) {
+        const int tq = (int)threadIdx.x / G, row = row0 + first_node + tq;
+        s_row[threadIdx.x] = tq < ntok ? row : -1;
+        s_lo[threadIdx.x] = p.window > 0 && tq < ntok ? p.row_pos[row] - p.window + 1 : INT_MIN;
+    }
     // the queries, while the first keys are on their way
-    for (int i = threadIdx.x; i < ROWS * (D / PER); i += kThreads) {
+    for (int i = threadIdx.x; i < ROWS * (D / PER); i += THREADS) {
         const int r = i / (D / PER), d = (i - r * (D / PER)) * PER;
         const int tq = r / G, hg = r - tq * G;
         vec v;
@@ -265,78 +254,107 @@ tree_attention_kernel(TreeArgs p, TreeSplit sp) {
         *(vec *)(qs + r * QP + d) = v;
     }
     __builtin_amdgcn_sched_barrier(0);       // loads come back in order: the scores do not wait for the values
-    if (kb < end) load_values(kb, pg);
+    if (kb < end) {
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++) load_values(kb, pg, dt);
+    }
     __syncthreads();
     unsigned bad = pg.bad;
     // a block's scores, weights and products; the next block's keys and values are asked for as soon as this one's are used
     auto block = [&](auto whole_block) __attribute__((always_inline)) {
         constexpr bool WHOLE = decltype(whole_block)::value;
-        const int next = kb + kWaves * KB;
-        bf16x8_t pb[NT][2];
-        f32x4_t pf[NT][TILES];
+        const int next = kb + KW * KB;
+        f32x4_t s[NT][TILES];
         unsigned long long any = 0;      // the slots that a row sees
+        bool grown = false;
+        // a block with nodes: their bits and positions come while the scores are made
+        Words words[NT];
+        int at = INT_MIN;
+        if constexpr (!WHOLE) {
+            if (kb + KB > kept) {
 #pragma unroll
-        for (int t = 0; t < NT; t++) {
-            f32x4_t s[TILES];
+                for (int t = 0; t < NT; t++) words[t] = words_of(t, kb);
+                const int j = kb - kept + lane;
+                if (p.window > 0 && lane < KB && j >= 0 && j < nodes) at = p.row_pos[row0 + j];
+            }
+        }
 #pragma unroll
-            for (int k = 0; k < TILES; k++) s[k] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+        for (int t = 0; t < NT; t++)
 #pragma unroll
-            for (int j = 0; j < KD; j++) {
-                const vec qv = *(const vec *)(qs + (t * 16 + c) * QP + (4 * j + g) * PER);
+            for (int k = 0; k < TILES; k++) s[t][k] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < KD; j++) {
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                const vec qv = *(const vec *)(qs + (at_row + t * 16) * QP + (4 * j + g) * PER);
 #pragma unroll
                 for (int k = 0; k < TILES; k++) {
                     if constexpr (kHalf) {
-                        s[k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[k][j], qv, s[k], 0, 0, 0);
+                        s[t][k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[k][j], qv, s[t][k], 0, 0, 0);
                     } else {
 #pragma unroll
-                        for (int e = 0; e < 4; e++) s[k] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[k][j][e], qv[e], s[k], 0, 0, 0);
+                        for (int e = 0; e < 4; e++) s[t][k] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[k][j][e], qv[e], s[t][k], 0, 0, 0);
                     }
                 }
             }
+            load_keys(next, pg, j);      // behind the last block: page 0, for nobody
+        }
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
             if constexpr (!WHOLE) {
-                unsigned long long bits = sight(t, kb, bad);
+                unsigned long long bits = sight(t, kb, bad, words[t], at);
                 any |= bits;
                 bits >>= 4 * g;
 #pragma unroll
                 for (int k = 0; k < TILES; k++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) s[k][i] = bits >> (16 * k + i) & 1 ? s[k][i] : -INFINITY;
+                    for (int i = 0; i < 4; i++) s[t][k][i] = bits >> (16 * k + i) & 1 ? s[t][k][i] : -INFINITY;
             }
             float top = -INFINITY;
 #pragma unroll
             for (int k = 0; k < TILES; k++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) top = fmaxf(top, s[k][i]);
-            top = max_32_apart(max_16_apart(top));
-            // The reference point follows the maximum only when that has grown by more than 2^8 in the exponent's units: until then
-            // weights are at most 256 times their final size, which sums and operands hold as well, and nothing is rescaled.
-            const float m_new = top > m_run[t] + tau ? top : m_run[t];
-            const float mc = m_new == -INFINITY ? 0.f : m_new * sc;       // nothing seen yet: exp2(-inf) = 0
-            if (__any(m_new != m_run[t])) {
-                const float alpha = exp2_fast(m_run[t] * sc - mc);
+                for (int i = 0; i < 4; i++) top = fmaxf(top, s[t][k][i]);
+            grown |= top > m_run[t] + tau;
+        }
+        // The reference point follows the maximum only when that has grown by more than 2^8 in the exponent's units: until then weights are
+        // at most 256 times their final size, which sums and operands hold as well, nothing is rescaled and no lane asks another.
+        if (__any(grown)) {
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                float top = -INFINITY;
+#pragma unroll
+                for (int k = 0; k < TILES; k++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) top = fmaxf(top, s[t][k][i]);
+                top = max_32_apart(max_16_apart(top));
+                const float m_new = top > m_run[t] + tau ? top : m_run[t];
+                const float alpha = exp2_fast((m_run[t] - m_new) * sc);
                 l_run[t] *= alpha;
 #pragma unroll
                 for (int dt = 0; dt < DT; dt++) o[t][dt] *= alpha;
                 m_run[t] = m_new;
             }
+        }
+        vec pv[NT][H];        // the weights as the second product takes them
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            const float mc = WHOLE ? m_run[t] * sc : fmaxf(m_run[t] * sc, kNothing);      // finite for a row that has seen nothing
             float sum = 0.f;
 #pragma unroll
             for (int k = 0; k < TILES; k++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    s[k][i] = exp2_fast(fmaf(s[k][i], sc, -mc));
-                    sum += s[k][i];
+                    s[t][k][i] = exp2_fast(fmaf(s[t][k][i], sc, -mc));
+                    sum += s[t][k][i];
                 }
             l_run[t] += sum;
-            if constexpr (kHalf) {
-                pb[t][0] = neighbours(pack8(s[0], s[1]));       // a weight is rounded to bfloat16 where it meets the value
-                pb[t][1] = neighbours(pack8(s[2], s[3]));
-            } else {
 #pragma unroll
-                for (int k = 0; k < TILES; k++) pf[t][k] = s[k];
+            for (int h = 0; h < H; h++) {
+                if constexpr (kHalf) pv[t][h] = neighbours(pack8(s[t][2 * h], s[t][2 * h + 1]));      // rounded to bfloat16 where they meet the values
+                else pv[t][h] = s[t][h];
             }
         }
-        if (next < end) load_keys(next, pg);
         if constexpr (!WHOLE) {
             // Slots that nobody sees may hold anything, and weights of zero do not keep a NaN or an infinity out: they are cleared.
             // So is what is not finite and only some rows see; those rows are given it at the end.
@@ -344,7 +362,7 @@ tree_attention_kernel(TreeArgs p, TreeSplit sp) {
             for (int step = 8; step > 0; step >>= 1) any |= __shfl_xor(any, step);
             unsigned odd = 0;
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
+            for (int h = 0; h < H; h++) {
                 const unsigned mine = (unsigned)(any >> (4 * PER * h + PER * g));
                 u32x4_t keep;
 #pragma unroll
@@ -363,7 +381,7 @@ tree_attention_kernel(TreeArgs p, TreeSplit sp) {
             if (__any((odd & kSigns) != 0)) {
                 if (lane == 0) s_odd = 1;
 #pragma unroll
-                for (int h = 0; h < 2; h++)
+                for (int h = 0; h < H; h++)
 #pragma unroll
                     for (int dt = 0; dt < DT; dt++) {
                         u32x4_t v = __builtin_bit_cast(u32x4_t, vf[h][dt]);
@@ -377,25 +395,26 @@ tree_attention_kernel(TreeArgs p, TreeSplit sp) {
             }
         }
 #pragma unroll
-        for (int t = 0; t < NT; t++)
+        for (int dt = 0; dt < DT; dt++) {
 #pragma unroll
-            for (int dt = 0; dt < DT; dt++)
+            for (int t = 0; t < NT; t++)
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
+                for (int h = 0; h < H; h++) {
                     if constexpr (kHalf) {
-                        o[t][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[h][dt], pb[t][h], o[t][dt], 0, 0, 0);
+                        o[t][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[h][dt], pv[t][h], o[t][dt], 0, 0, 0);
                     } else {
 #pragma unroll
-                        for (int e = 0; e < 4; e++) o[t][dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[h][dt][e], pf[t][h][e], o[t][dt], 0, 0, 0);
+                        for (int e = 0; e < 4; e++) o[t][dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[h][dt][e], pv[t][h][e], o[t][dt], 0, 0, 0);
                     }
                 }
-        if (next < end) load_values(next, pg);
+            load_values(next, pg, dt);
+        }
         kb = next;
         bad = pg.bad;
-        pg = block_pages(kb + kWaves * KB);
+        pg = block_pages(kb + KW * KB);
     };
     if (kb < end) {
-        pg = block_pages(kb + kWaves * KB);
+        pg = block_pages(kb + KW * KB);
         const int whole_end = min(kept, end) - KB;
         do {
         while (kb >= lo_max && kb <= whole_end && bad == 0) block(std::true_type());      // slots that every row sees
@@ -404,18 +423,47 @@ tree_attention_kernel(TreeArgs p, TreeSplit sp) {
         } while (kb < end);
     }
 
-    // The waves saw different slots: their statistics and outputs meet, four neighbouring outputs a thread.
+    // The groups saw different slots: their statistics and outputs meet, four neighbouring outputs a thread.
+    __syncthreads();      // the queries have been read
+    const int met = max(1, min(KW, (end - begin + KB - 1) / KB));        // groups that had slots
+    auto put_outputs = [&](int at) {
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            if (g == 0) {
+                sm_m[kw * ROWS + at_row + t * 16] = m_run[t];
+                sm_l[kw * ROWS + at_row + t * 16] = l_run[t];
+            }
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++) *(f32x4_t *)(sm_o + (at * ROWS + at_row + t * 16) * OP + dt * 16 + 4 * g) = o[t][dt];
+        }
+    };
 #pragma unroll
     for (int t = 0; t < NT; t++) {
-        const float l = sum_32_apart(sum_16_apart(l_run[t]));
-        if (g == 0) {
-            sm_m[wave * ROWS + t * 16 + c] = m_run[t] == -INFINITY ? -INFINITY : m_run[t] * sc;      // in the exponent's units from here on
-            sm_l[wave * ROWS + t * 16 + c] = l;
-        }
+        l_run[t] = sum_32_apart(sum_16_apart(l_run[t]));
+        m_run[t] = m_run[t] == kNothing ? -INFINITY : m_run[t] * sc;      // in the exponent's units from here on
+    }
+    if constexpr (WT < KW) {      // half of the groups at a time, for want of room
+        if (kw >= WT && kw < met) put_outputs(kw - WT);
+        __syncthreads();
+        if (kw + WT < met) {
 #pragma unroll
-        for (int dt = 0; dt < DT; dt++) *(f32x4_t *)(sm_o + (wave * ROWS + t * 16 + c) * OP + dt * 16 + 4 * g) = o[t][dt];
+            for (int t = 0; t < NT; t++) {
+                const float m1 = sm_m[(kw + WT) * ROWS + at_row + t * 16], m = fmaxf(m_run[t], m1);
+                const float f0 = m_run[t] == -INFINITY ? 0.f : exp2_fast(m_run[t] - m), f1 = m1 == -INFINITY ? 0.f : exp2_fast(m1 - m);
+                m_run[t] = m;
+                l_run[t] = l_run[t] * f0 + sm_l[(kw + WT) * ROWS + at_row + t * 16] * f1;
+#pragma unroll
+                for (int dt = 0; dt < DT; dt++)
+                    o[t][dt] = o[t][dt] * f0 + *(const f32x4_t *)(sm_o + (kw * ROWS + at_row + t * 16) * OP + dt * 16 + 4 * g) * f1;
+            }
+        }
+        __syncthreads();
+        if (kw < min(WT, met)) put_outputs(kw);
+    } else if (kw < met) {
+        put_outputs(kw);
     }
     __syncthreads();
+    const int parts_here = min(WT, met);
     const int live_rows = ntok * G;
     const size_t group = ((size_t)seg * p.kv_heads + kvh) * sp.tiles + tile;
     constexpr int PART = ROWS * (D + 4);      // floats of a part: outputs, then a maximum and a sum a row (four words a row)
@@ -431,15 +479,13 @@ tree_attention_kernel(TreeArgs p, TreeSplit sp) {
         if constexpr (kHalf) *(bf16x4_t *)dst = (bf16x4_t){v[0], v[1], v[2], v[3]};
         else *(f32x4_t *)dst = (f32x4_t){v[0], v[1], v[2], v[3]};
     };
-    for (int idx = threadIdx.x; idx < live_rows * (D / 4); idx += kThreads) {
+    for (int idx = threadIdx.x; idx < live_rows * (D / 4); idx += THREADS) {
         const int r = idx / (D / 4), d = (idx - r * (D / 4)) * 4;
         float m = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < kWaves; w++) m = fmaxf(m, sm_m[w * ROWS + r]);
+        for (int w = 0; w < parts_here; w++) m = fmaxf(m, sm_m[w * ROWS + r]);
         float l = 0.f;
         f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int w = 0; w < kWaves; w++) {
+        for (int w = 0; w < parts_here; w++) {
             const float mw = sm_m[w * ROWS + r], f = mw == -INFINITY ? 0.f : exp2_fast(mw - m);
             l += sm_l[w * ROWS + r] * f;
             acc += *(const f32x4_t *)(sm_o + (w * ROWS + r) * OP + d) * f;
@@ -448,10 +494,8 @@ tree_attention_kernel(TreeArgs p, TreeSplit sp) {
             // Values that are not finite reach the rows that see them here: slot by slot, as the plain kernel would.
             const int row = row0 + first_node + r / G, lo = p.window > 0 ? p.row_pos[row] - p.window + 1 : INT_MIN;
             for (int slot = begin; slot < end; slot++) {
-                const int j = slot - kept, page = p.tables[(size_t)seg * p.table_stride + (slot >> PSH)];
-                const bool sees = (unsigned)page < (unsigned)p.num_pages &&
-                                  (j < 0 ? slot >= lo : (j >> 6) < p.words && (p.seen[(size_t)row * p.words + (j >> 6)] >> (j & 63) & 1) && p.row_pos[row0 + j] >= lo);
-                if (!sees) continue;
+                if (!sees_slot<PSH>(p, seg, row0, kept, row, lo, slot)) continue;
+                const int page = p.tables[(size_t)seg * p.table_stride + (slot >> PSH)];
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const float v = (float)((const T *)p.vp)[(((size_t)page * nkv + kvh) * D + d + i) * PS + (slot & PMASK)];
@@ -480,101 +524,62 @@ tree_attention_kernel(TreeArgs p, TreeSplit sp) {
     if (threadIdx.x == 0) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);   // for the next launch
     const unsigned base = (unsigned)(group * sp.splits * PART * sizeof(float));
     constexpr unsigned kStep = PART * sizeof(float);
-    float *factor = sm_o;                          // [live][ROWS]; the parts' shares of a row
-    for (int i = threadIdx.x; i < live * live_rows; i += kThreads) {
-        const int s = i / live_rows, r = i - s * live_rows;
-        const f32x4_t ml = take_over(meet, base + s * kStep + (unsigned)(ROWS * D + r * 4) * 4);
-        factor[s * ROWS + r] = ml[0];
-        factor[(live + s) * ROWS + r] = ml[1];
-    }
-    __syncthreads();
-    for (int r = threadIdx.x; r < live_rows; r += kThreads) {
+    // Eight parts at a time, their statistics and two pieces of their outputs in one trip; later ones move the maximum as slots do.
+    for (int idx = threadIdx.x; idx < live_rows * (D / 8); idx += THREADS) {
+        const int r = idx / (D / 8), d = (idx - r * (D / 8)) * 4;
         float m = -INFINITY, l = 0.f;
-        for (int s = 0; s < live; s++) m = fmaxf(m, factor[s * ROWS + r]);
-        for (int s = 0; s < live; s++) {
-            const float ms = factor[s * ROWS + r], f = ms == -INFINITY ? 0.f : exp2_fast(ms - m);
-            factor[s * ROWS + r] = f;
-            l += factor[(live + s) * ROWS + r] * f;
-        }
-        sm_m[r] = m;
-        sm_l[r] = l;
-    }
-    __syncthreads();
-    for (int idx = threadIdx.x; idx < live_rows * (D / 4); idx += kThreads) {
-        const int r = idx / (D / 4), d = (idx - r * (D / 4)) * 4;
-        f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
-        for (int s0 = 0; s0 < live; s0 += 8) {       // eight loads on their way at a time
-            f32x4_t part[8];
+        f32x4_t acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+        for (int s0 = 0; s0 < live; s0 += 8) {
+            f32x4_t ml[8], part[2][8];
 #pragma unroll
-            for (int i = 0; i < 8; i++) part[i] = take_over(meet, base + min(s0 + i, live - 1) * kStep + (unsigned)(r * D + d) * 4);
+            for (int i = 0; i < 8; i++) {
+                const unsigned from = base + min(s0 + i, live - 1) * kStep;
+                ml[i] = take_over(meet, from + (unsigned)(ROWS * D + r * 4) * 4);
+                part[0][i] = take_over(meet, from + (unsigned)(r * D + d) * 4);
+                part[1][i] = take_over(meet, from + (unsigned)(r * D + d + D / 2) * 4);
+            }
+            float m_new = m;
 #pragma unroll
-            for (int i = 0; i < 8; i++)
-                if (s0 + i < live) acc += part[i] * factor[(s0 + i) * ROWS + r];
+            for (int i = 0; i < 8; i++) m_new = fmaxf(m_new, ml[i][0]);
+            const float f = m == -INFINITY ? 0.f : exp2_fast(m - m_new);
+            l *= f;
+            acc[0] *= f;
+            acc[1] *= f;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                if (s0 + i >= live) break;
+                const float w = ml[i][0] == -INFINITY ? 0.f : exp2_fast(ml[i][0] - m_new);
+                l += ml[i][1] * w;
+                acc[0] += part[0][i] * w;
+                acc[1] += part[1][i] * w;
+            }
+            m = m_new;
         }
-        finish(r, d, acc, sm_m[r], sm_l[r]);
+        finish(r, d, acc[0], m, l);
+        finish(r, d + D / 2, acc[1], m, l);
     }
 }
 
-constexpr int kMostSplits = 64;
-
-// Parts of the slots: as many as fill the device, and a round of the waves each at least.
-void plan_splits(long groups, int slots_of_device, int round, int max_context, size_t part_bytes, size_t room, TreeSplit *sp) {
-    const long span = (long)max_context + round;      // the first part starts on a block, at or below the first slot
-    long want = groups > 0 ? slots_of_device / groups : 1;
-    want = std::max(1l, std::min(want, (long)kMostSplits));
-    want = std::min(want, (span + round - 1) / round);
-    if (part_bytes * (size_t)groups > 0) want = std::min(want, (long)(room / (part_bytes * (size_t)groups)));
-    want = std::max(want, 1l);
-    sp->per = (int)(((span + want - 1) / want + round - 1) / round * round);
-    sp->splits = (int)((span + sp->per - 1) / sp->per);
-}
-
-int compute_units() {
-    static int cus = 0;
-    if (cus == 0) {
-        int dev = 0, n = 0;
-        if (hipGetDevice(&dev) == hipSuccess) (void)hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev);
-        cus = n > 0 ? n : 256;
-    }
-    return cus;
-}
-
-template <typename T, int D, int NT, int PSH, int EU>
+template <typename T, int D, int NT, int PSH, int H, int RG, int KW, int EU>
 int launch(const TreeArgs &a, int max_context, hipStream_t stream) {
-    constexpr size_t smem = lds_bytes<T, D, NT>();
-    static_assert(smem + 16 <= 160 * 1024, "more than a compute unit's LDS");
-    // the parts' shares of the rows lie where the outputs of the waves were
-    static_assert((size_t)2 * kMostSplits * 16 * NT <= (size_t)kWaves * 16 * NT * (D + 4), "the shares of all parts do not fit");
-    const int G = a.heads / a.kv_heads, TQ = 16 * NT / G;
+    constexpr int W = RG * KW, ROWS = 16 * NT * RG;
+    constexpr size_t smem = lds_bytes<T, D, ROWS, KW>();
+    static_assert(smem + 8 * ROWS + 16 <= 160 * 1024, "more than a compute unit's LDS");
+    const int G = a.heads / a.kv_heads, TQ = ROWS / G;
     TreeSplit sp;
     sp.tiles = (a.max_nodes + TQ - 1) / TQ;
-    sp.negate = a.scale < 0.f;
-    sp.scale = (a.scale < 0.f ? -a.scale : a.scale) * kLog2e;
-    sp.counters = nullptr;
-    sp.parts = nullptr;
-    const long groups = (long)a.num_segs * a.kv_heads * sp.tiles;
-    void *ws = nullptr;
-    size_t ws_bytes = 0;
-    const int round = kWaves * 16 * Operand<T>::kTiles;
-    constexpr size_t part_bytes = (size_t)16 * NT * (D + 4) * sizeof(float);
-    sp.splits = 1;
-    sp.per = 1 << 28;
-    const int context = (int)std::min({(long)max_context, (long)a.table_stride * a.page_size, 1l << 28});      // the last part takes what is left
-    if (groups * (long)sizeof(int) <= (long)kWorkspaceCounterBytes && fllm_device_workspace(&ws, &ws_bytes) && ws_bytes > kWorkspaceCounterBytes) {
-        plan_splits(groups, compute_units() * (int)std::min((size_t)EU, (160 * 1024) / smem), round, context, part_bytes,
-                    std::min(ws_bytes - kWorkspaceCounterBytes, (size_t)0x7fffffff), &sp);
-        sp.counters = (int *)ws;
-        sp.parts = (float *)((unsigned char *)ws + kWorkspaceCounterBytes);
-    }
+    constexpr int round = KW * H * Operand<T>::kStep;
+    constexpr size_t part_bytes = (size_t)ROWS * (D + 4) * sizeof(float);
+    plan_tree(a, sp.tiles, compute_units() * (int)std::min((size_t)(4 * EU / W), (160 * 1024) / smem), round, 4, max_context, part_bytes, &sp);
     const long units = (long)a.num_segs * sp.splits * a.kv_heads, blocks = (units + 7) / 8 * 8 * sp.tiles;
     FLLM_REQUIRE(blocks <= 0x7fffffffL, "tree_attention: grid too large");
     static bool raised = false;      // more than the default 64 KiB of dynamic LDS has to be asked for once
     if (!raised) {
-        const hipError_t e = hipFuncSetAttribute((const void *)tree_attention_kernel<T, D, NT, PSH, EU>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        const hipError_t e = hipFuncSetAttribute((const void *)tree_attention_kernel<T, D, NT, PSH, H, RG, KW, EU>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         FLLM_REQUIRE(e == hipSuccess, "tree_attention: cannot raise the LDS limit: %s", hipGetErrorString(e));
         raised = true;
     }
-    hipLaunchKernelGGL((tree_attention_kernel<T, D, NT, PSH, EU>), dim3((unsigned)blocks), dim3(kThreads), smem, stream, a, sp);
+    hipLaunchKernelGGL((tree_attention_kernel<T, D, NT, PSH, H, RG, KW, EU>), dim3((unsigned)blocks), dim3(W * kWave), smem, stream, a, sp);
     return fllm_check_launch("tree_attention");
 }
 
@@ -582,20 +587,34 @@ template <typename T, int D>
 int launch_rows(const TreeArgs &a, int max_context, hipStream_t stream) {
     const int G = a.heads / a.kv_heads;
     const long rows = (long)a.max_nodes * G;
-    auto go = [&](auto nt, auto eu) {
-        constexpr int NT = decltype(nt)::value, EU = decltype(eu)::value;
-        if (a.page_size == 8) return launch<T, D, NT, 3, EU>(a, max_context, stream);
-        if (a.page_size == 16) return launch<T, D, NT, 4, EU>(a, max_context, stream);
-        if (a.page_size == 32) return launch<T, D, NT, 5, EU>(a, max_context, stream);
-        return launch<T, D, NT, 6, EU>(a, max_context, stream);
+    auto go = [&](auto nt, auto rg, auto kw) {
+        constexpr int NT = decltype(nt)::value, RG = decltype(rg)::value, KW = decltype(kw)::value;
+        if (a.page_size == 8) return launch<T, D, NT, 3, 1, RG, KW, 2>(a, max_context, stream);
+        if (a.page_size == 16) return launch<T, D, NT, 4, 1, RG, KW, 2>(a, max_context, stream);
+        if (a.page_size == 32) return launch<T, D, NT, 5, 1, RG, KW, 2>(a, max_context, stream);
+        return launch<T, D, NT, 6, 1, RG, KW, 2>(a, max_context, stream);
     };
-    using std::integral_constant;
-    if (rows <= 16 && G <= 16) return go(integral_constant<int, 1>(), integral_constant<int, 2>());
+    using one = std::integral_constant<int, 1>;
+    using two = std::integral_constant<int, 2>;
+    using four = std::integral_constant<int, 4>;
+    using eight = std::integral_constant<int, 8>;
+    if (rows <= 16 && G <= 16) return go(one(), one(), eight());
     if constexpr (sizeof(T) == 4) {
-        return go(integral_constant<int, 2>(), integral_constant<int, D == 128 ? 1 : 2>());
+        return go(two(), one(), eight());
     } else {
-        if (rows <= 32 && G <= 32) return go(integral_constant<int, 2>(), integral_constant<int, D == 128 ? 1 : 2>());
-        return go(integral_constant<int, 4>(), integral_constant<int, D == 128 ? 1 : 2>());
+        // Tiles of 32 rows while they fit the device side by side, of 64 where there are more of them; heads of 128 over long contexts go to
+        // the kernel whose rows share every key through LDS.  Microseconds at 32 heads on 8, tiles of 32 / of 64 / shared, 8 requests of up to
+        // 26 nodes (256 tiles of 32) at 1,000, 2,000, 4,000, 8,000 kept tokens: 14.2 / 20.1 / 22.8, 23.6 / 29.5 / 33.1, 40.5 / 46.6 / 41.7,
+        // 72.8 / 78.2 / 58.6; of up to 64 nodes (512): 25.3 / 20.4 / 30.3, 38.7 / 36.2 / 38.5, 64.0 / 66.0 / 54.0, 118 / 128 / 89.
+        // Heads of 64, 32 requests of up to 64 nodes at 6,144: 174 / 132 / 149.
+        const int per = 32 / G > 0 ? 32 / G : 1;
+        const long tiles = (long)a.num_segs * a.kv_heads * ((a.max_nodes + per - 1) / per);
+        const int asked = fllm_option_tree_rows();
+        const bool far = asked ? asked == 128 : tiles * reach_of(a, max_context) > 1500000;
+        if (G <= 32 && (asked ? asked == 32 : tiles <= compute_units() && !far)) return go(two(), one(), eight());
+        if constexpr (D == 64) return go(four(), one(), eight());
+        else if (far) return fllm_tree_attention_wide(a, max_context, stream);
+        else return go(two(), two(), four());
     }
 }
 

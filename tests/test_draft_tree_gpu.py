@@ -98,13 +98,18 @@ def test_what_a_row_does_not_see_does_not_reach_it(ops, dim, heads, kv_heads, dt
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
-def test_what_a_row_sees_does_reach_it(ops, dtype):
-    case = plain.TreeCase([(100, 12)], 4, 2, 64, 16, dtype, seed=3)
+@pytest.mark.parametrize("dim,rows", [(64, 0), (128, 0), (128, 64), (128, 128), (64, 64)])
+def test_what_a_row_sees_does_reach_it(ops, dim, rows, dtype):
+    case = plain.TreeCase([(100, 12)], 4, 2, dim, 16, dtype, seed=3)
+    ops.set_option("attention.tree_rows", rows)
     case.seen_of[0] = [{0, i} for i in range(12)]
     for j, value in ((1, float("nan")), (2, float("inf")), (3, float("-inf"))):
         case.values[0][100 + j] = value
         case.put(0, 100 + j)
-    got = attend(ops, case, 0.125).float().cpu()
+    try:
+        got = attend(ops, case, 0.125).float().cpu()
+    finally:
+        ops.set_option("attention.tree_rows", 0)
     assert bool(torch.isnan(got[1]).all()) and bool((got[2] == float("inf")).all()) and bool((got[3] == float("-inf")).all())
     assert bool(torch.isfinite(got[[0] + list(range(4, 12))]).all())
 
@@ -137,6 +142,23 @@ def test_the_plain_kernel_and_the_fast_one(ops, plain_kernels):
         check(ops, case, sinks=True)
     finally:
         ops.set_fast_kernels(True)
+
+
+@pytest.mark.parametrize("rows", [32, 64, 128])
+@pytest.mark.parametrize("heads,kv_heads,dim,page", [(8, 2, 128, 16), (8, 1, 128, 8), (14, 2, 128, 32), (36, 2, 128, 64), (8, 2, 64, 16), (40, 2, 64, 8), (8, 8, 128, 64)])
+def test_tiles_of_any_number_of_rows(ops, rows, heads, kv_heads, dim, page):
+    """What the launch chooses by the number of tiles and the reach of their rows, asked for by hand."""
+    ops.set_option("attention.tree_rows", rows)
+    try:
+        case = plain.TreeCase(RAGGED + [(900, 70)], heads, kv_heads, dim, page, torch.bfloat16, seed=rows + dim + page, spare_rows=2)
+        check(ops, case)
+        check(ops, case, window=50, sinks=True)
+        check(ops, case, scale=-0.1)
+        case = plain.TreeCase([(3000, 30), (1, 90)], heads, kv_heads, dim, page, torch.bfloat16, seed=rows + dim)
+        assert torch.equal(check(ops, case, sinks=True), check(ops, case, sinks=True))
+        test_what_a_row_does_not_see_does_not_reach_it(ops, dim, heads, kv_heads, torch.bfloat16)
+    finally:
+        ops.set_option("attention.tree_rows", 0)
 
 
 # ---- the walk --------------------------------------------------------------------------------------------------------------
