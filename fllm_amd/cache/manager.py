@@ -156,6 +156,37 @@ class CacheManager:
         dst.length = pages * page_size
         return dst.length
 
+    def fork_request(self, src_id, dst_id) -> List[Optional[tuple]]:
+        """For a request `dst_id` that holds nothing yet: it goes on from what `src_id` has committed.  Full pages are held by both (neither
+        writes them again: each writes at and behind its committed length); of a page that is partly filled `dst_id` gets one of its own.
+        Returns for every group the (page of `src_id`, page of `dst_id`) whose contents the caller copies before either request's next
+        step, or None where the length ends on a page's edge.  Raises `OutOfPages` and changes nothing where a group has no page left.
+        Windows: what a window has given up stays given up in both."""
+        src, dst = self._get(src_id), self._get(dst_id)
+        if src is dst or dst.length != 0 or any(dst.tables):
+            raise ValueError(f"request {dst_id!r} already holds tokens")
+        partial = [src.length % group.page_size != 0 for group in self.groups]
+        for g, needed in enumerate(partial):
+            if needed and self.free_pages(g) < 1:
+                raise OutOfPages(f"group {g} needs 1 page, 0 are free")
+        for g, needed in enumerate(partial):
+            self._make_room(g, 1 if needed else 0)
+        copies: List[Optional[tuple]] = []
+        for g, group in enumerate(self.groups):
+            full = src.length // group.page_size
+            for page in src.tables[g][:full]:
+                if page >= 0:
+                    self.pools[g].retain(page)
+                dst.tables[g].append(page)
+            copies.append(None)
+            if partial[g]:
+                dst.tables[g].append(self.pools[g].alloc())
+                copies[g] = (src.tables[g][full], dst.tables[g][full])
+        for node in src.shared:
+            self._hold(dst, node)
+        dst.length = src.length
+        return copies
+
     def remember_prefix(self, req_id, tokens: Sequence[int], known: Optional[int] = None) -> None:
         """Enters the full pages of a request into the index.  `tokens` are the request's tokens from its first on, of
         which the first `known` are final; pages wholly below that and below the committed length are entered.  Where

@@ -27,6 +27,17 @@ class CacheBinding:
 
 
 @dataclass
+class TreeRows:
+    """What a step on trees of drafted tokens says beside its positions: a node's row lies in the slot kept + its number, and sees the
+    kept tokens and the nodes whose bits are set (`Ops.tree_attention`)."""
+    row_slot: torch.Tensor                  # int32 [R]
+    kept: torch.Tensor                      # int32 [S]
+    seen: torch.Tensor                      # int64 [R, words]
+    parents: torch.Tensor                   # int32 [R]: node numbers, for the walk along the model's choices
+    max_nodes: int
+
+
+@dataclass
 class StepContext:
     num_rows: int
     num_segments: int
@@ -51,6 +62,7 @@ class StepContext:
     then_norm: object = None
     next_norm: object = None
     prepared: object = None
+    tree: Optional[TreeRows] = None         # rows are nodes of trees of drafted tokens (mixers that say `takes_trees`)
     step_values: Dict[str, torch.Tensor] = field(default_factory=dict)   # what a layer leaves for later layers of the same step
     _scratch: Dict = field(default_factory=dict)
 

@@ -21,7 +21,7 @@ from ..config.spec import ModelSpec
 from ..parts.runtime import Runtime
 from ..registry import model_spec_from_config
 from ..weights.loader import check_tensors, load_checkpoint
-from .context import StepContext
+from .context import StepContext, TreeRows
 from .model import Model
 
 _DTYPES = {"float32": torch.float32, "fp32": torch.float32, "f32": torch.float32,
@@ -58,6 +58,15 @@ class StepEntry:
     tokens: Sequence[int]
     want: Sequence[int] = ()
     carry: Optional[int] = None
+
+
+@dataclass
+class TreeEntry:
+    """A tree of drafted tokens behind a request's committed ones: tokens[0] is the request's newest token (which no step has computed yet),
+    every other node continues the node `parents` names, of a lower number (parents[0] does not count)."""
+    req_id: object
+    tokens: Sequence[int]
+    parents: Sequence[int]
 
 
 class ModelRunner:
@@ -110,6 +119,7 @@ class ModelRunner:
                                                               max_step_tokens=self.max_step_tokens)
         self.steps = 0
         self.rows_total = 0
+        self._tree: Optional[tuple] = None         # the last step's trees, until `keep_tree` or another step
         # decode steps replay captured graphs when every part can be captured (parts say so with
         # `graph_safe`; a part that decides on the host per step cannot)
         parts_ok = all(getattr(b.mixer, "graph_safe", False)
@@ -174,10 +184,31 @@ class ModelRunner:
         return self.cache.add_request(req_id)
 
     def free_request(self, req_id) -> None:
+        if self._tree is not None and any(e.req_id == req_id for e in self._tree[0]):
+            self._tree = None
         self.cache.free_request(req_id)
 
     def length(self, req_id) -> int:
         return self.cache.length(req_id)
+
+    def fork_request(self, src_id, dst_id) -> None:
+        """`dst_id` (which must not hold a cache) goes on from what `src_id` has committed: full pages are held by both, a page that is
+        partly filled and the state of fixed size are copied.  Raises `OutOfPages` and changes nothing where the room is not there."""
+        self.cache.length(src_id)                  # an unknown request is refused before anything is added
+        self.cache.add_request(dst_id)
+        try:
+            copies = self.cache.fork_request(src_id, dst_id)
+        except Exception:
+            self.cache.free_request(dst_id)
+            raise
+        for g, copy in enumerate(copies):
+            if copy is None:
+                continue
+            stores = [t for t in (self.model.k_store[g], self.model.v_store[g], *(self.model.pool_store[g] or ())) if t.numel() > 0]
+            self.rt.ops.copy_pages(stores, [copy[0]], [copy[1]])
+        src, dst = self.cache.slot(src_id), self.cache.slot(dst_id)
+        for _, _, arena in self.model.state_arenas():
+            arena[dst].copy_(arena[src])
 
     # ---- the step -------------------------------------------------------------------------
     def _validate(self, entries: Sequence[StepEntry], previous_tokens: Optional[torch.Tensor] = None) -> None:
@@ -233,6 +264,7 @@ class ModelRunner:
         Raises `OutOfPages` (nothing changed) when the pages do not suffice.
         `previous_tokens`: the int32 device tensor that entries with `carry` take their token from."""
         self._validate(entries, previous_tokens)
+        self._tree = None
         added = []
         try:
             for e in entries:
@@ -269,6 +301,91 @@ class ModelRunner:
         self.steps += 1
         self.rows_total += sum(len(e.tokens) for e in entries)
         return logits
+
+    # ---- trees of drafted tokens ------------------------------------------------------------
+    def step_tree(self, entries: Sequence[TreeEntry]) -> torch.Tensor:
+        """Runs trees of drafted tokens as one batch and returns float32 logits [nodes, vocab], entry by entry and node by node: each node's
+        in the context of the request's committed tokens and the nodes from the root to it.  Nothing is committed: `keep_tree` keeps the
+        nodes that the model chose itself; any other step leaves the trees behind.  For models whose layers all attend over pages
+        without a chunk, normed heads or biased scores, and keep no state."""
+        if not all(getattr(self.model.blocks[e.layer].mixer, "takes_trees", False) for e in self.spec.run_order) or self.model.has_state:
+            raise StepError("a layer of this model cannot attend over trees of drafted tokens")
+        from ..kernels import tree_rows
+        rows = []
+        for e in entries:
+            if len(e.parents) != len(e.tokens):
+                raise StepError(f"request {e.req_id!r} brings {len(e.tokens)} nodes and {len(e.parents)} parents")
+            try:
+                rows.append(tree_rows(e.parents))
+            except ValueError as exc:
+                raise StepError(f"request {e.req_id!r}: {exc}") from None
+        self._validate([StepEntry(e.req_id, e.tokens) for e in entries])
+        for e in entries:
+            if not self.cache.has_request(e.req_id):
+                raise StepError(f"request {e.req_id!r} holds no cache: its prompt is not a tree")
+        need = [0] * len(self.cache.groups)
+        for e in entries:
+            for g, m in enumerate(self.cache.pages_missing(e.req_id, self.cache.length(e.req_id) + len(e.tokens))):
+                need[g] += m
+        for g, n in enumerate(need):
+            if n > self.cache.free_pages(g):
+                raise OutOfPages(f"the step needs {n} pages of cache group {g}, {self.cache.free_pages(g)} are free")
+        for e in entries:
+            self.cache.reserve(e.req_id, self.cache.length(e.req_id) + len(e.tokens))
+        total = sum(len(e.tokens) for e in entries)
+        ctx = self._build_context([StepEntry(e.req_id, e.tokens, range(len(e.tokens))) for e in entries])
+        # segments of one row lie behind the others: the trees follow the segments
+        order = sorted(range(len(entries)), key=lambda i: len(entries[i].tokens) == 1)
+        words = max(len(seen[0]) for _, seen in rows)
+        slots, positions, parents, seen, kept = [], [], [], [], []
+        for i in order:
+            start, (depths, bits) = self.cache.length(entries[i].req_id), rows[i]
+            kept.append(start)
+            slots.extend(range(start, start + len(depths)))
+            positions.extend(start + d for d in depths)
+            parents.extend([-1] + [int(p) for p in entries[i].parents[1:]])
+            seen.extend(b + [0] * (words - len(b)) for b in bits)
+        packed = torch.tensor(slots + positions + parents + kept, dtype=torch.int32, device=self.device)
+        ctx.row_pos = packed[total:2 * total]
+        ctx.tree = TreeRows(row_slot=packed[:total], kept=packed[3 * total:], seen=torch.tensor(seen, dtype=torch.int64, device=self.device),
+                            parents=packed[2 * total:3 * total], max_nodes=max(len(e.tokens) for e in entries))
+        logits = self.model.forward(ctx)
+        self._tree = (list(entries), order, ctx, 1 + max(max(depths) for depths, _ in rows))
+        self.steps += 1
+        self.rows_total += total
+        return logits
+
+    def keep_tree(self, chosen: torch.Tensor) -> List[tuple]:
+        """After `step_tree`: `chosen` (int32 [nodes], on the device, in the order of the logits) is the token that the model chose behind every
+        node.  Follows the choices from each root to the last node that was drafted, moves the walked nodes' keys and values up behind
+        the committed tokens, commits them and gives back the other nodes' pages.  Returns for every entry (the walked nodes, the
+        request's newest token: what was chosen at the last of them)."""
+        if self._tree is None:
+            raise StepError("keep_tree follows a step_tree")
+        entries, order, ctx, most = self._tree
+        rows = sum(len(e.tokens) for e in entries)
+        if chosen.shape != (rows,):
+            raise StepError(f"{rows} nodes were computed, {tuple(chosen.shape)} tokens are given")
+        ops, S = self.rt.ops, len(entries)
+        if order != list(range(S)):               # the logits have the order of the entries, the rows that of the segments
+            starts = [0]
+            for e in entries:
+                starts.append(starts[-1] + len(e.tokens))
+            chosen = chosen[torch.tensor([r for i in order for r in range(starts[i], starts[i + 1])], device=self.device)]
+        path = torch.empty((S, most), dtype=torch.int32, device=self.device)
+        ends = torch.empty((2, S), dtype=torch.int32, device=self.device)
+        ops.follow_tree(ctx.ids, ctx.tree.parents, ctx.seg_start, chosen.contiguous(), path, ends[0], ends[1])
+        for g, table in enumerate(ctx.tables):
+            v_store = self.model.v_store[g]
+            ops.move_tokens(self.model.k_store[g], v_store if v_store.numel() > 0 else None, table, ctx.tree.kept, path, ends[0])
+        self._tree = None
+        walked, (lengths, newest) = path.tolist(), ends.tolist()
+        out: List[Optional[tuple]] = [None] * S
+        for s, i in enumerate(order):
+            self.cache.commit(entries[i].req_id, lengths[s])
+            self.cache.trim(entries[i].req_id, self.cache.length(entries[i].req_id))
+            out[i] = (walked[s][: lengths[s]], newest[s])
+        return out
 
     # ---- decode steps as HIP graphs ---------------------------------------------------------
     def _graph_step(self, entries: Sequence[StepEntry], previous_tokens: Optional[torch.Tensor] = None

@@ -89,12 +89,16 @@ class PagedAttention(Mixer):
         if self.gated and self.qk_norm_eps is None:
             raise ValueError("an output gate rides in the product of a layer with normed heads: ask for qk_norm_eps too")
         self.sink = rt.vector(weights["sink"]) if spec.get("sink", False) else None
+        # whether a step's rows may be nodes of trees of drafted tokens: not with a chunk of positions, normed heads (their store knows no
+        # slots) or scores that a position encoding biases
+        self.takes_trees = self.chunk is None and self.qk_norm_eps is None
         position = spec.get("position")
         self.position = None
         if position is not None:
             position = dict(position)
             kind = position.pop("kind")
             self.position = part_class("position", kind)(PartSpec(kind, position), {}, rt)
+            self.takes_trees = self.takes_trees and getattr(self.position, "score_slopes", None) is None
         # Rotary with the checkpoint's pairing (l, l + dims/2): the rows of the q and k projections are
         # reordered inside every head so that the partners sit next to each other (2l, 2l + 1), the
         # pairing the kernels rotate.  q . k does not change when both are reordered alike
@@ -178,7 +182,8 @@ class PagedAttention(Mixer):
             cos, sin, dims, pairing = ctx.no_rotation(rt)
         ops.rope_kv_store(qkv, ctx.row_pos, ctx.row_seg, tables, cos, sin,
                           binding.k_pages if binding.writes else None, binding.v_pages if binding.writes else None,
-                          nh, nkv, d, dims, pairing, binding.page_size, **self.shape_args)
+                          nh, nkv, d, dims, pairing, binding.page_size, **self.shape_args,
+                          **({} if ctx.tree is None else {"row_slot": ctx.tree.row_slot}))
         self._attend_and_project(ctx, qkv[:, : nh * d], residual, binding, branch=branch)
 
     def forward_from_residual(self, ctx, residual, norm, binding, branch=None) -> bool:
@@ -188,7 +193,7 @@ class PagedAttention(Mixer):
         rows = residual.shape[0]
         prologue = getattr(norm, "fused_prologue", lambda: None)()
         form = fused_form(ops, rows, self.hidden, self.w_qkv) if hasattr(ops, "norm_qkv_rope_store") else None
-        if prologue is None or form is None or not self.takes_prepared:
+        if prologue is None or form is None or not self.takes_prepared or ctx.tree is not None:      # the fused store puts a row at its position
             return False
         norm_scale, norm_eps = prologue
         nh, nkv, d = self.heads, self.kv_heads, self.head_dim
@@ -237,7 +242,11 @@ class PagedAttention(Mixer):
         if 0 < single_from < ctx.num_segments and ctx.single_max_context < self.SPLIT_SINGLE_ROWS_FROM:
             single_from = ctx.num_segments
         slopes = getattr(self.position, "score_slopes", None)      # a position encoding may bias scores by distance
-        if slopes is not None:
+        if ctx.tree is not None:
+            ops.tree_attention(q, binding.k_pages, binding.v_pages, tables, ctx.row_pos, ctx.seg_start, ctx.tree.kept, ctx.tree.seen, out, nh, nkv, d,
+                               binding.page_size, self.scale, ctx.max_context, window=self.window, sinks=self.sink,
+                               max_nodes=ctx.tree.max_nodes, **self.shape_args)
+        elif slopes is not None:
             ops.attention(q, binding.k_pages, binding.v_pages, tables, ctx.row_pos, ctx.row_seg, ctx.seg_start,
                           out, nh, nkv, d, binding.page_size, self.scale, self.window, ctx.max_context, head_slopes=slopes,
                           **shape_args)

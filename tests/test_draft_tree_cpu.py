@@ -95,3 +95,97 @@ def test_pages_that_are_not_copied():
     for source, target in ((10, 1), (1, 10), (-1, 1), (1, -1), (3, 3)):
         assert call(source, target) != 0 and "of 10" in lib.fllm_last_error().decode()
     assert call(1, 2, 9) != 0 and "9 stores" in lib.fllm_last_error().decode()
+
+
+# ---- a request that goes on in two ways -------------------------------------------------------------------------------------
+def group(window=None, page_size=4):
+    from fllm_amd.cache import GroupSpec
+    return GroupSpec(entries=(0,), kv_heads=2, k_dim=16, v_dim=16, window=window, page_size=page_size)
+
+
+def test_a_fork_holds_full_pages_and_copies_the_last():
+    from fllm_amd.cache import CacheManager, OutOfPages
+    m = CacheManager([group(), group(window=6)], [6, 6], max_requests=4)
+    m.add_request("a"), m.reserve("a", 14), m.commit("a", 10)
+    m.add_request("b")
+    copies = m.fork_request("a", "b")
+    assert m.length("b") == 10 and len(m.table("b", 0)) == 3 and len(m.table("a", 0)) == 4
+    assert m.table("b", 0)[:2] == m.table("a", 0)[:2] and copies[0] == (m.table("a", 0)[2], m.table("b", 0)[2]) and copies[0][0] != copies[0][1]
+    assert m.table("b", 1)[0] == m.table("a", 1)[0] == -1 and m.table("b", 1)[1] == m.table("a", 1)[1] and copies[1][0] == m.table("a", 1)[2]
+    m.check_invariants()
+    m.add_request("c")
+    with pytest.raises(OutOfPages):                       # a group without a page: nothing is changed
+        m.reserve("a", 17), m.fork_request("a", "c")
+    assert m.length("c") == 0 and m.table("c", 0) == [] and m.table("c", 1) == []
+    m.check_invariants()
+    m.free_request("a")
+    m.reserve("b", 11), m.commit("b", 1)
+    m.check_invariants()
+    for wrong in (("b", "b"), ("c", "b")):
+        with pytest.raises(ValueError):
+            m.fork_request(*wrong)
+    with pytest.raises(KeyError):
+        m.fork_request("nobody", "c")
+    m.free_request("b"), m.free_request("c")
+    assert m.free_pages(0) == 6 and m.free_pages(1) == 6
+    m.check_invariants()
+
+
+def test_a_fork_on_a_pages_edge_and_of_nothing():
+    from fllm_amd.cache import CacheManager
+    m = CacheManager([group()], [4], max_requests=3)
+    m.add_request("a"), m.reserve("a", 8), m.commit("a", 8)
+    m.add_request("b")
+    assert m.fork_request("a", "b") == [None] and m.table("b", 0) == m.table("a", 0) and m.free_pages() == 2
+    m.add_request("c"), m.free_request("b"), m.add_request("b")
+    assert m.fork_request("c", "b") == [None] and m.length("b") == 0
+    m.check_invariants()
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_forks_in_random_orders_keep_the_books(seed):
+    from fllm_amd.cache import CacheManager, OutOfPages
+    rng = random.Random(seed)
+    prefixes = seed % 2 == 0
+    m = CacheManager([group()] if prefixes else [group(), group(window=7)], [30] if prefixes else [30, 30], max_requests=6)
+    if prefixes:
+        m.enable_prefix_cache()
+    tokens, number, forks = {}, 0, 0
+    for _ in range(500):
+        what = rng.random()
+        if what < 0.2 and len(tokens) < 6:
+            m.add_request(number)
+            tokens[number] = [rng.randrange(2) for _ in range(40)]
+            if prefixes:
+                m.adopt_prefix(number, tokens[number][:20])
+            number += 1
+        elif what < 0.45 and tokens and len(tokens) < 6:
+            src = rng.choice(list(tokens))
+            m.add_request(number)
+            try:
+                copies = m.fork_request(src, number)
+                tokens[number] = list(tokens[src])
+                forks += 1
+                assert [c is not None for c in copies] == [m.length(src) % 4 != 0] * len(m.groups)
+            except OutOfPages:
+                m.free_request(number)
+            number += 1
+        elif what < 0.85 and tokens:
+            r = rng.choice(list(tokens))
+            n = min(rng.randint(1, 9), 40 - m.length(r))
+            if n and m.can_reserve(r, m.length(r) + n):
+                m.reserve(r, m.length(r) + n)
+                m.commit(r, rng.randint(0, n))
+                if rng.random() < 0.5:
+                    m.trim(r, m.length(r))
+                if prefixes:
+                    m.remember_prefix(r, tokens[r][: m.length(r)])
+        elif tokens:
+            r = rng.choice(list(tokens))
+            m.free_request(r)
+            del tokens[r]
+        m.check_invariants()
+    assert forks > 10
+    for r in tokens:
+        m.free_request(r)
+    m.check_invariants()
