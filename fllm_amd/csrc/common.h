@@ -40,7 +40,7 @@ int fllm_option_half_tiles(void);
 int fllm_option_wide_waves(void);
 int fllm_option_resident_tiles(void);
 int fllm_option_tile32_rows(void);
-// rows of a tile of tree attention in bfloat16: 0 (chosen by the launch), 32, 64 or 128 (heads of 64: 64)
+// rows of a tile of tree attention: 0 (chosen by the launch), 16, 32, 64 or 128 (heads of 64: 64, float32: 32 at most)
 int fllm_option_tree_rows(void);
 // 1: decode-shaped products of up to 8 rows use 8-row weight tiles with two K halves a product (default); 0: 16-row tiles
 int fllm_option_dual_k(void);

@@ -43,7 +43,7 @@ static int g_resident_tiles = 1;  // q/k/v of up to 16 rows behind a prepared no
 int fllm_option_resident_tiles(void) { return g_resident_tiles; }
 static int g_half_tiles = 1;      // products of many rows: a last round that is half full at most runs as tiles of half the rows; 0 never, 2 wherever it can
 int fllm_option_half_tiles(void) { return g_half_tiles; }
-static int g_tree_rows = 0;       // rows of a tile of tree attention in bfloat16, 0: chosen by the launch
+static int g_tree_rows = 0;       // rows of a tile of tree attention, 0: chosen by the launch
 int fllm_option_tree_rows(void) { return g_tree_rows; }
 static int g_slab = 1;
 int fllm_option_slab(void) { return g_slab; }
@@ -76,7 +76,7 @@ extern "C" int fllm_set_option(const char *name, int value) {
         return 0;
     }
     if (strcmp(name, "attention.tree_rows") == 0) {
-        g_tree_rows = (value == 32 || value == 64 || value == 128) ? value : 0;
+        g_tree_rows = (value == 16 || value == 32 || value == 64 || value == 128) ? value : 0;
         return 0;
     }
     if (strcmp(name, "linear.resident_tiles") == 0) {

@@ -66,7 +66,8 @@ constexpr size_t lds_bytes() {
 
 // H: value loads of all lanes a block, 32 slots (float32: 16) each.
 // PSH: pages of 1 << PSH tokens; of 8, two a score tile, otherwise of 16, 32 or 64.
-template <typename T, int D, int NT, int PSH, int H, int RG, int KW, int EU>
+// ALONE: no other tile reads the same keys.
+template <typename T, int D, int NT, int PSH, int H, int RG, int KW, int EU, bool ALONE>
 __global__ void __launch_bounds__(RG * KW * kWave) __attribute__((amdgpu_waves_per_eu(EU, EU)))
 tree_attention_kernel(TreeArgs p, TreeSplit sp) {
     typedef typename Operand<T>::vec vec;
@@ -143,15 +144,33 @@ tree_attention_kernel(TreeArgs p, TreeSplit sp) {
     vec kf[TILES][KD], vf[H][DT];
     // A lane's place in a page is the same in every block; the rest of an address is a scalar wherever one page serves all lanes.
     constexpr size_t kHeadBytes = (size_t)D * PS * sizeof(T);
-    const unsigned k_lane = kHalf ? (unsigned)(g * PS + (P8 ? c & 7 : c)) * 16 : (unsigned)((g >> 1) * PS + (P8 ? c & 7 : c)) * 32 + (g & 1) * 16;
+    // Rows of the score tiles.  A tile alone reads a key once, from memory: row c of score tile k is slot 16 k + c, a load is whole lines, carries
+    // the non-temporal hint, and probabilities change lanes for it.  Where several tiles read the same keys most come from L2, and what
+    // counts is the instructions: row c of score tile k of a step of 32 slots is slot 8 (c / 4) + 4 (k % 2) + c % 4, so that a lane's
+    // scores are of the neighbouring slots that its values are of.  Microseconds with one order and the hint / with the other: 8 requests
+    // of 8 nodes at 16,000 kept tokens 62 / 75; of 26 nodes at 2,000 (4 tiles a key/value head) 23.6 / 19.8.
+    constexpr bool kSwap = kHalf && ALONE, kNear = kHalf && !ALONE;
+    const int k_token = kNear ? (P8 ? c & 3 : PSH == 4 ? (c & 3) + 8 * (c >> 2 & 1) : (c & 3) + 8 * (c >> 2)) : P8 ? c & 7 : c;
+    const unsigned k_lane = kHalf ? (unsigned)(g * PS + k_token) * 16 : (unsigned)((g >> 1) * PS + k_token) * 32 + (g & 1) * 16;
     // piece j of a block's keys
     auto load_keys = [&](int kb, const Pages &pg, int j) __attribute__((always_inline)) {
+        const size_t page_bytes = (size_t)nkv * kHeadBytes;
 #pragma unroll
         for (int t = 0; t < TILES; t++) {
-            const char *base = (const char *)p.kp + (size_t)kvh * kHeadBytes + (P8 ? 0 : (size_t)((kb + 16 * t) & PMASK) * (8 * sizeof(T)));
-            if (P8) base += (size_t)(c < 8 ? pg.page[P8 ? 2 * t : t] : pg.page[P8 ? 2 * t + 1 : t]) * nkv * kHeadBytes;
-            else base += (size_t)pg.page[t] * nkv * kHeadBytes;
-            kf[t][j] = __builtin_nontemporal_load((const vec *)(base + j * 64 * PS + k_lane));
+            const char *base = (const char *)p.kp + (size_t)kvh * kHeadBytes;
+            if constexpr (kNear) {
+                const int h = t >> 1;
+                if constexpr (P8) base += (size_t)(c < 8 ? (c < 4 ? pg.page[4 * h] : pg.page[4 * h + 1]) : (c < 12 ? pg.page[4 * h + 2] : pg.page[4 * h + 3])) * page_bytes;
+                else if constexpr (PSH == 4) base += (size_t)(c < 8 ? pg.page[2 * h] : pg.page[2 * h + 1]) * page_bytes;
+                else base += (size_t)pg.page[2 * h] * page_bytes + (size_t)((kb + 32 * h) & PMASK) * 16;
+                base += (t & 1) * 64;
+            } else {
+                if constexpr (P8) base += (size_t)(c < 8 ? pg.page[2 * t] : pg.page[2 * t + 1]) * page_bytes;
+                else base += (size_t)pg.page[t] * page_bytes + (size_t)((kb + 16 * t) & PMASK) * (8 * sizeof(T));
+            }
+            const vec *from = (const vec *)(base + j * 64 * PS + k_lane);
+            if constexpr (ALONE) kf[t][j] = __builtin_nontemporal_load(from);
+            else kf[t][j] = *from;
         }
     };
     // values: bfloat16 the slots 32 h + 8 g .. + 7, float32 16 h + 4 g .. + 3
@@ -304,11 +323,11 @@ tree_attention_kernel(TreeArgs p, TreeSplit sp) {
             if constexpr (!WHOLE) {
                 unsigned long long bits = sight(t, kb, bad, words[t], at);
                 any |= bits;
-                bits >>= 4 * g;
+                bits >>= kNear ? 8 * g : 4 * g;
 #pragma unroll
                 for (int k = 0; k < TILES; k++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) s[t][k][i] = bits >> (16 * k + i) & 1 ? s[t][k][i] : -INFINITY;
+                    for (int i = 0; i < 4; i++) s[t][k][i] = bits >> (kNear ? 32 * (k >> 1) + 4 * (k & 1) + i : 16 * k + i) & 1 ? s[t][k][i] : -INFINITY;
             }
             float top = -INFINITY;
 #pragma unroll
@@ -351,7 +370,8 @@ tree_attention_kernel(TreeArgs p, TreeSplit sp) {
             l_run[t] += sum;
 #pragma unroll
             for (int h = 0; h < H; h++) {
-                if constexpr (kHalf) pv[t][h] = neighbours(pack8(s[t][2 * h], s[t][2 * h + 1]));      // rounded to bfloat16 where they meet the values
+                if constexpr (kSwap) pv[t][h] = neighbours(pack8(s[t][2 * h], s[t][2 * h + 1]));
+                else if constexpr (kHalf) pv[t][h] = pack8(s[t][2 * h], s[t][2 * h + 1]);      // rounded to bfloat16 where they meet the values
                 else pv[t][h] = s[t][h];
             }
         }
@@ -560,7 +580,7 @@ tree_attention_kernel(TreeArgs p, TreeSplit sp) {
     }
 }
 
-template <typename T, int D, int NT, int PSH, int H, int RG, int KW, int EU>
+template <typename T, int D, int NT, int PSH, int H, int RG, int KW, int EU, bool ALONE>
 int launch(const TreeArgs &a, int max_context, hipStream_t stream) {
     constexpr int W = RG * KW, ROWS = 16 * NT * RG;
     constexpr size_t smem = lds_bytes<T, D, ROWS, KW>();
@@ -570,16 +590,16 @@ int launch(const TreeArgs &a, int max_context, hipStream_t stream) {
     sp.tiles = (a.max_nodes + TQ - 1) / TQ;
     constexpr int round = KW * H * Operand<T>::kStep;
     constexpr size_t part_bytes = (size_t)ROWS * (D + 4) * sizeof(float);
-    plan_tree(a, sp.tiles, compute_units() * (int)std::min((size_t)(4 * EU / W), (160 * 1024) / smem), round, 4, max_context, part_bytes, &sp);
+    plan_tree(a, sp.tiles, compute_units() * (int)std::min((size_t)(4 * EU / W), (160 * 1024) / smem), round, sizeof(T) == 4 ? 1 : 4, max_context, part_bytes, &sp);
     const long units = (long)a.num_segs * sp.splits * a.kv_heads, blocks = (units + 7) / 8 * 8 * sp.tiles;
     FLLM_REQUIRE(blocks <= 0x7fffffffL, "tree_attention: grid too large");
     static bool raised = false;      // more than the default 64 KiB of dynamic LDS has to be asked for once
     if (!raised) {
-        const hipError_t e = hipFuncSetAttribute((const void *)tree_attention_kernel<T, D, NT, PSH, H, RG, KW, EU>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        const hipError_t e = hipFuncSetAttribute((const void *)tree_attention_kernel<T, D, NT, PSH, H, RG, KW, EU, ALONE>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         FLLM_REQUIRE(e == hipSuccess, "tree_attention: cannot raise the LDS limit: %s", hipGetErrorString(e));
         raised = true;
     }
-    hipLaunchKernelGGL((tree_attention_kernel<T, D, NT, PSH, H, RG, KW, EU>), dim3((unsigned)blocks), dim3(W * kWave), smem, stream, a, sp);
+    hipLaunchKernelGGL((tree_attention_kernel<T, D, NT, PSH, H, RG, KW, EU, ALONE>), dim3((unsigned)blocks), dim3(W * kWave), smem, stream, a, sp);
     return fllm_check_launch("tree_attention");
 }
 
@@ -589,31 +609,48 @@ int launch_rows(const TreeArgs &a, int max_context, hipStream_t stream) {
     const long rows = (long)a.max_nodes * G;
     auto go = [&](auto nt, auto rg, auto kw) {
         constexpr int NT = decltype(nt)::value, RG = decltype(rg)::value, KW = decltype(kw)::value;
-        if (a.page_size == 8) return launch<T, D, NT, 3, 1, RG, KW, 2>(a, max_context, stream);
-        if (a.page_size == 16) return launch<T, D, NT, 4, 1, RG, KW, 2>(a, max_context, stream);
-        if (a.page_size == 32) return launch<T, D, NT, 5, 1, RG, KW, 2>(a, max_context, stream);
-        return launch<T, D, NT, 6, 1, RG, KW, 2>(a, max_context, stream);
+        const bool alone = a.max_nodes <= 16 * NT * RG / G;
+        auto of_page = [&](auto psh) {
+            constexpr int PSH = decltype(psh)::value;
+            if constexpr (RG == 1 && NT < 4) {
+                if (alone) return launch<T, D, NT, PSH, 1, RG, KW, 2, true>(a, max_context, stream);
+            }
+            return launch<T, D, NT, PSH, 1, RG, KW, 2, false>(a, max_context, stream);
+        };
+        if (a.page_size == 8) return of_page(std::integral_constant<int, 3>());
+        if (a.page_size == 16) return of_page(std::integral_constant<int, 4>());
+        if (a.page_size == 32) return of_page(std::integral_constant<int, 5>());
+        return of_page(std::integral_constant<int, 6>());
     };
     using one = std::integral_constant<int, 1>;
     using two = std::integral_constant<int, 2>;
     using four = std::integral_constant<int, 4>;
     using eight = std::integral_constant<int, 8>;
-    if (rows <= 16 && G <= 16) return go(one(), one(), eight());
+    // Tiles of 16 rows while every one of them has a compute unit and the keys that they read again are few: a tile's fixed cost (its waves meet
+    // in LDS) goes with its rows.  Microseconds in tiles of 16 / of 32 at 32 heads on 8: a request of 8 nodes at 250, 1,000, 4,000 kept tokens
+    // 7.3 / 9.5, 9.8 / 11.9, 12.4 / 16.4, of 26 nodes at 1,000, 4,000, 8,000 10.4 / 12.2, 13.6 / 14.5, 19.2 / 18.5; 8 of 16 at 1,000 and 4,000
+    // 11.4 / 13.7 and 27.5 / 26.1.
+    const long pairs = (long)a.num_segs * a.kv_heads;
+    const auto tiles_of = [&](int height) { return height < G ? LONG_MAX / 4 : pairs * ((a.max_nodes + height / G - 1) / (height / G)); };
+    const long reach = reach_of(a, max_context);
+    const bool cold = pairs * reach * D * 2 * (long)sizeof(T) > (256l << 20);        // more than the last cache holds
+    const int asked = fllm_option_tree_rows();
+    const long tiles16 = tiles_of(16);
+    if (G <= 16 && (asked ? asked == 16 : rows <= 16 || (tiles16 <= compute_units() && !cold && (sizeof(T) == 4 || tiles16 * reach <= 600000))))
+        return go(one(), one(), eight());
     if constexpr (sizeof(T) == 4) {
         return go(two(), one(), eight());
     } else {
-        // Tiles of 32 rows while they fit the device side by side, of 64 where there are more of them; heads of 128 over long contexts go to
-        // the kernel whose rows share every key through LDS.  Microseconds at 32 heads on 8, tiles of 32 / of 64 / shared, 8 requests of up to
-        // 26 nodes (256 tiles of 32) at 1,000, 2,000, 4,000, 8,000 kept tokens: 14.2 / 20.1 / 22.8, 23.6 / 29.5 / 33.1, 40.5 / 46.6 / 41.7,
-        // 72.8 / 78.2 / 58.6; of up to 64 nodes (512): 25.3 / 20.4 / 30.3, 38.7 / 36.2 / 38.5, 64.0 / 66.0 / 54.0, 118 / 128 / 89.
-        // Heads of 64, 32 requests of up to 64 nodes at 6,144: 174 / 132 / 149.
-        const int per = 32 / G > 0 ? 32 / G : 1;
-        const long tiles = (long)a.num_segs * a.kv_heads * ((a.max_nodes + per - 1) / per);
-        const int asked = fllm_option_tree_rows();
-        const bool far = asked ? asked == 128 : tiles * reach_of(a, max_context) > 1500000;
-        if (G <= 32 && (asked ? asked == 32 : tiles <= compute_units() && !far)) return go(two(), one(), eight());
+        // Tiles of 32 rows while they fit the device side by side, of 64 where there are more of them.  Heads of 128 go to the kernel whose
+        // rows share every key through LDS where there are more tiles than that, or where the keys and values of all requests are more than
+        // the last cache holds (256 MB): tiles that read them again then read memory again.  Microseconds at 32 heads on 8, tiles of 32 / of 64 /
+        // shared: 8 requests of up to 26 nodes (256 tiles of 32) at 1,000, 4,000, 16,000 kept tokens (393 MB) 12.9 / 18.3 / 24.0,
+        // 30.0 / 33.3 / 39.1, 146 / 152 / 109; of up to 64 nodes (512) at 1,000, 4,000, 16,000 23.9 / 19.2 / 29.2, 48.7 / 45.3 / 54.1,
+        // 223 / 227 / 169; 32 requests of up to 64 nodes at 1,000 84.7 / 61.3 / 47.1.  Heads of 64, tiles of 32 / of 64: 8 requests of up to 26
+        // nodes at 1,000 and 8,000 9.2 / 13.5 and 28.8 / 32.1, of up to 64 nodes 16.4 / 13.9 and 48.7 / 46.5.
+        if (G <= 32 && (asked ? asked <= 32 : rows <= 32 || (tiles_of(32) <= compute_units() && !cold))) return go(two(), one(), eight());
         if constexpr (D == 64) return go(four(), one(), eight());
-        else if (far) return fllm_tree_attention_wide(a, max_context, stream);
+        else if (asked ? asked == 128 : cold || tiles_of(64) > 2 * compute_units()) return fllm_tree_attention_wide(a, max_context, stream);
         else return go(two(), two(), four());
     }
 }

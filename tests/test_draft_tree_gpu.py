@@ -144,7 +144,7 @@ def test_the_plain_kernel_and_the_fast_one(ops, plain_kernels):
         ops.set_fast_kernels(True)
 
 
-@pytest.mark.parametrize("rows", [32, 64, 128])
+@pytest.mark.parametrize("rows", [16, 32, 64, 128])
 @pytest.mark.parametrize("heads,kv_heads,dim,page", [(8, 2, 128, 16), (8, 1, 128, 8), (14, 2, 128, 32), (36, 2, 128, 64), (8, 2, 64, 16), (40, 2, 64, 8), (8, 8, 128, 64)])
 def test_tiles_of_any_number_of_rows(ops, rows, heads, kv_heads, dim, page):
     """What the launch chooses by the number of tiles and the reach of their rows, asked for by hand."""
