@@ -277,15 +277,16 @@ def _dense(t: torch.Tensor, name: str, dtype=None, shape=None) -> None:
 def _here(t: torch.Tensor, name: str, device: int) -> None:
     if not t.is_cuda:
         raise KernelError(f"{name} must be on the GPU")
-    if t.device.index != device:
-        raise KernelError(f"{name} is on device {t.device.index}, the current device is {device}")
+    if t.get_device() != device:
+        raise KernelError(f"{name} is on device {t.get_device()}, the current device is {device}")
 
 
-def _held(t: torch.Tensor, name: str, device: int, dtype, shape) -> None:
-    """As `_dense`, and on the current device."""
-    if t.device.index != device or t.dtype != dtype or t.shape != shape or not t.is_contiguous():
+def _held(t: torch.Tensor, name: str, device: int, dtype, shape) -> int:
+    """As `_dense`, and on the current device; its address."""
+    if t.dtype is not dtype or t.get_device() != device or t.shape != shape or not t.is_contiguous():
         _dense(t, name, dtype, shape)
         _here(t, name, device)
+    return t.data_ptr()
 
 
 def tree_rows(parents: Sequence[int], words: Optional[int] = None) -> Tuple[list, list]:
@@ -476,15 +477,16 @@ class Ops:
         return stream.device_index, stream.cuda_stream
 
     @staticmethod
-    def _current_device() -> int:
-        return Ops._current_stream()[0]
-
-    @staticmethod
     def _stream() -> int:
         """The current stream.  Kernels of one device meet in that device's workspace (counters that each launch leaves
         at zero, partial results behind them), so launches on one device must not overlap: all of them go to one stream
         (a stream that is capturing a graph stands for the stream the graph will be replayed on).  A launch on a second
         stream of the same device is refused."""
+        return Ops._stream_and_device()[0]
+
+    @staticmethod
+    def _stream_and_device() -> Tuple[int, int]:
+        """What `_stream` gives, and the device it is of."""
         device, handle = Ops._current_stream()
         seen = Ops._streams.get(device)
         if seen is None:
@@ -493,7 +495,7 @@ class Ops:
         elif handle != seen and not torch.cuda.is_current_stream_capturing():
             raise KernelError(f"kernels of device {device} were launched on stream {seen:#x} before and are now asked for on "
                               f"stream {handle:#x}: they share the device workspace and must stay on one stream")
-        return handle
+        return handle, device
 
     @staticmethod
     def _on_the_kernels_stream() -> bool:
@@ -2058,37 +2060,31 @@ class Ops:
         `q` may be a column slice of a wider matrix; `v_dim`, `key_chunk` as in `attention`; `out` has memory of its own.
         `max_context` bounds kept + nodes over the segments, `max_nodes` (64 * words where it is not given) the nodes: a segment's rows
         beyond it are left as they are."""
-        rows = q.shape[0]
+        _need(q.dim() == 2 and tables.dim() == 2 and seen.dim() == 2, "q must be [rows, lanes], tables [segments, pages], seen [rows, words]")
+        rows, width = q.shape
         v_dim = head_dim if v_dim is None else int(v_dim)
-        device = self._current_device()
-        _need(q.is_cuda and q.dim() == 2 and q.stride(1) == 1 and q.shape[1] == heads * head_dim,
-              f"q must be [rows, {heads * head_dim}] with unit column stride")
+        stream, device = self._stream_and_device()
         dtype = q.dtype
-        _need(dtype in _DTYPE_CODE, f"dtype {dtype} unsupported")
+        if not (q.is_cuda and q.stride(1) == 1 and width == heads * head_dim):
+            raise KernelError(f"q must be [rows, {heads * head_dim}] with unit column stride")
+        if dtype not in _DTYPE_CODE:
+            raise KernelError(f"dtype {dtype} unsupported")
         _need(key_chunk > 0 and head_dim % key_chunk == 0, "tree_attention: bad chunk of key values")
         _here(q, "q", device)
         num_pages = k_pages.shape[0]
-        _held(k_pages, "k_pages", device, dtype, (num_pages, kv_heads, head_dim // key_chunk, page_size, key_chunk))
-        _held(v_pages, "v_pages", device, dtype, (num_pages, kv_heads, v_dim, page_size))
-        _need(tables.dim() == 2, "tables must be [segments, pages]")
         segs, stride = tables.shape
-        _held(tables, "tables", device, torch.int32, (segs, stride))
-        _held(row_pos, "row_pos", device, torch.int32, (rows,))
-        _held(seg_start, "seg_start", device, torch.int32, (segs + 1,))
-        _held(kept, "kept", device, torch.int32, (segs,))
-        _need(seen.dim() == 2 and seen.shape[1] > 0, "seen must be [rows, words]")
-        words = seen.shape[1]
-        _held(seen, "seen", device, torch.int64, (rows, words))
-        _held(out, "out", device, dtype, (rows, heads * v_dim))
-        if sinks is not None:
-            _held(sinks, "sinks", device, torch.float32, (heads,))
+        _, words = seen.shape
         most = 64 * words if max_nodes is None else int(max_nodes)
-        _need(0 <= most <= 64 * words, f"max_nodes {most}: {words} words hold the bits of at most {64 * words}")
+        if not 0 <= most <= 64 * words or words == 0:
+            raise KernelError(f"max_nodes {most}: {words} words hold the bits of at most {64 * words}")
         self._check(self.lib.fllm_tree_attention(
-            _ptr(q), q.stride(0) if rows > 1 else heads * head_dim, _ptr(k_pages), _ptr(v_pages), _ptr(tables), stride, _ptr(row_pos),
-            _ptr(seg_start), segs, _ptr(kept), _ptr(seen), words, _ptr(out), rows, heads, kv_heads, head_dim, v_dim, page_size, num_pages,
-            float(scale), int(window) if window else 0, key_chunk, _ptr(sinks), _DTYPE_CODE[dtype], min(most, rows), int(max_context),
-            self._stream()))
+            q.data_ptr(), q.stride(0) if rows > 1 else width, _held(k_pages, "k_pages", device, dtype, (num_pages, kv_heads, head_dim // key_chunk, page_size, key_chunk)),
+            _held(v_pages, "v_pages", device, dtype, (num_pages, kv_heads, v_dim, page_size)), _held(tables, "tables", device, torch.int32, (segs, stride)), stride,
+            _held(row_pos, "row_pos", device, torch.int32, (rows,)), _held(seg_start, "seg_start", device, torch.int32, (segs + 1,)), segs,
+            _held(kept, "kept", device, torch.int32, (segs,)), _held(seen, "seen", device, torch.int64, (rows, words)), words,
+            _held(out, "out", device, dtype, (rows, heads * v_dim)), rows, heads, kv_heads, head_dim, v_dim, page_size, num_pages,
+            float(scale), int(window) if window else 0, key_chunk, None if sinks is None else _held(sinks, "sinks", device, torch.float32, (heads,)),
+            _DTYPE_CODE[dtype], min(most, rows), int(max_context), stream))
         return out
 
     def follow_tree(self, drafted: torch.Tensor, parents: torch.Tensor, seg_start: torch.Tensor, chosen: torch.Tensor, path: torch.Tensor,
@@ -2098,20 +2094,15 @@ class Ops:
         the walk goes to the lowest child whose token is what was chosen at its parent.  `path` (int32 [segments, n], n the most nodes
         wanted): its nodes, -1 behind them; `length`: how many; `newest`: what was chosen at the last, the request's next token.  A
         segment without rows: length 0, newest -1."""
-        rows, segs = drafted.shape[0], seg_start.shape[0] - 1
-        device = self._current_device()
-        _need(drafted.dim() == 1 and seg_start.dim() == 1 and segs >= 0, "drafted must be [rows], seg_start [segments + 1]")
-        _held(drafted, "drafted", device, torch.int32, (rows,))
-        _held(parents, "parents", device, torch.int32, (rows,))
-        _held(chosen, "chosen", device, torch.int32, (rows,))
-        _held(seg_start, "seg_start", device, torch.int32, (segs + 1,))
-        _need(path.dim() == 2 and path.shape[1] > 0, "path must be [segments, nodes]")
-        most = path.shape[1]
-        _held(path, "path", device, torch.int32, (segs, most))
-        _held(length, "length", device, torch.int32, (segs,))
-        _held(newest, "newest", device, torch.int32, (segs,))
-        self._check(self.lib.fllm_follow_tree(_ptr(drafted), _ptr(parents), _ptr(seg_start), segs, _ptr(chosen), rows, _ptr(path), most,
-                                              _ptr(length), _ptr(newest), self._stream()))
+        stream, device = self._stream_and_device()
+        _need(drafted.dim() == 1 and path.dim() == 2, "drafted must be [rows], path [segments, nodes]")
+        (rows,), (segs, most), i32 = drafted.shape, path.shape, torch.int32
+        _need(most > 0, "path must have room for a node")
+        self._check(self.lib.fllm_follow_tree(
+            _held(drafted, "drafted", device, i32, (rows,)), _held(parents, "parents", device, i32, (rows,)),
+            _held(seg_start, "seg_start", device, i32, (segs + 1,)), segs, _held(chosen, "chosen", device, i32, (rows,)), rows,
+            _held(path, "path", device, i32, (segs, most)), most, _held(length, "length", device, i32, (segs,)),
+            _held(newest, "newest", device, i32, (segs,)), stream))
 
     def move_tokens(self, k_store: torch.Tensor, v_store: Optional[torch.Tensor], tables: torch.Tensor, kept: torch.Tensor, path: torch.Tensor,
                     length: torch.Tensor) -> None:
@@ -2120,54 +2111,56 @@ class Ops:
         `k_store` [layers, pages, kv_heads, k_dim / chunk, page_size, chunk] (or [layers, pages, kv_heads, page_size, k_dim]) and
         `v_store` [layers, pages, kv_heads, v_dim, page_size] (None where keys are all there is): the pages of all layers that share the
         block tables `tables` [segments, pages].  Slots without a page are left out."""
-        device = self._current_device()
-        _need(k_store.dim() in (5, 6), "k_store must be [layers, pages, kv_heads, k_dim / chunk, page_size, chunk]")
-        layers, pages, kv_heads = k_store.shape[:3]
-        page_size, chunk = k_store.shape[-2:]
-        k_dim = chunk * (k_store.shape[3] if k_store.dim() == 6 else 1)
-        _need(k_store.dtype in _DTYPE_CODE, f"dtype {k_store.dtype} unsupported")
-        _held(k_store, "k_store", device, k_store.dtype, k_store.shape)
+        stream, device = self._stream_and_device()
+        shape, dtype, i32 = k_store.shape, k_store.dtype, torch.int32
+        _need(len(shape) in (5, 6), "k_store must be [layers, pages, kv_heads, k_dim / chunk, page_size, chunk]")
+        if dtype not in _DTYPE_CODE:
+            raise KernelError(f"dtype {dtype} unsupported")
+        layers, pages, kv_heads = shape[:3]
+        page_size, chunk = shape[-2:]
         v_dim = 0
         if v_store is not None:
             _need(v_store.dim() == 5, "v_store must be [layers, pages, kv_heads, v_dim, page_size]")
             v_dim = v_store.shape[3]
-            _held(v_store, "v_store", device, k_store.dtype, (layers, pages, kv_heads, v_dim, page_size))
-        _need(tables.dim() == 2, "tables must be [segments, pages]")
-        segs, stride = tables.shape
-        _held(tables, "tables", device, torch.int32, (segs, stride))
-        _held(kept, "kept", device, torch.int32, (segs,))
-        _need(path.dim() == 2 and path.shape[1] > 0, "path must be [segments, nodes]")
-        _held(path, "path", device, torch.int32, (segs, path.shape[1]))
-        _held(length, "length", device, torch.int32, (segs,))
+        _need(tables.dim() == 2 and path.dim() == 2, "tables must be [segments, pages], path [segments, nodes]")
+        (segs, stride), (_, most) = tables.shape, path.shape
+        _need(most > 0, "path must have room for a node")
         self._check(self.lib.fllm_move_tokens(
-            _ptr(k_store), _ptr(v_store), layers, pages, kv_heads, k_dim, v_dim, page_size, chunk, k_store.element_size(), _ptr(tables), stride,
-            segs, _ptr(kept), _ptr(path), path.shape[1], _ptr(length), self._stream()))
+            _held(k_store, "k_store", device, dtype, shape),
+            None if v_store is None else _held(v_store, "v_store", device, dtype, (layers, pages, kv_heads, v_dim, page_size)),
+            layers, pages, kv_heads, chunk * (shape[3] if len(shape) == 6 else 1), v_dim, page_size, chunk, 4 if dtype is torch.float32 else 2,
+            _held(tables, "tables", device, i32, (segs, stride)), stride, segs, _held(kept, "kept", device, i32, (segs,)),
+            _held(path, "path", device, i32, (segs, most)), most, _held(length, "length", device, i32, (segs,)), stream))
 
     def copy_pages(self, stores: Sequence[torch.Tensor], source: Sequence[int], target: Sequence[int]) -> None:
         """Page source[i] is copied to page target[i] in every layer of every store ([layers, pages, ...], at most 8 of them): what a request
         takes over of another's when it goes on from the same tokens (`CacheManager.fork_request` names the pages), or a cache that is
         packed.  No page is a target twice, or a source and a target."""
-        device = self._current_device()
-        pairs = len(source)
-        _need(len(target) == pairs, f"{pairs} pages to copy from, {len(target)} to copy to")
-        _need(0 < len(stores) <= 8, f"{len(stores)} stores: 1 to 8 are copied at a time")
+        stream, device = self._stream_and_device()
+        pairs, count = len(source), len(stores)
+        if len(target) != pairs:
+            raise KernelError(f"{pairs} pages to copy from, {len(target)} to copy to")
+        if not 0 < count <= 8:
+            raise KernelError(f"{count} stores: 1 to 8 are copied at a time")
         targets = set(target)
         _need(len(targets) == pairs, "a page is copied to twice")
         _need(targets.isdisjoint(source), "a page is copied from and to")
-        sizes = []
+        lowest, highest = (min(min(source), min(target)), max(max(source), max(target))) if pairs else (0, -1)
+        addresses, sizes = [], []
         for n, store in enumerate(stores):
-            _need(store.dim() >= 2, f"store {n} must be [layers, pages, ...]")
-            _held(store, f"store {n}", device, store.dtype, store.shape)
-            pages = store.shape[1]
-            _need(pairs == 0 or (0 <= min(source) and max(source) < pages and 0 <= min(target) and max(target) < pages),
-                  f"store {n} has {pages} pages")
-            sizes.append((store.shape[0], pages, store[0, 0].numel() * store.element_size() if pages and store.shape[0] else 0))
+            shape = store.shape
+            if len(shape) < 2:
+                raise KernelError(f"store {n} must be [layers, pages, ...]")
+            addresses.append(_held(store, "a store", device, store.dtype, shape))
+            layers, pages = shape[:2]
+            if not (0 <= lowest and highest < pages):
+                raise KernelError(f"store {n} has {pages} pages")
+            sizes.append((layers, pages, store.numel() // max(1, layers * pages) * store.element_size()))
         if pairs == 0:
             return
-        counts = [(ctypes.c_int64 * len(stores))(*column) for column in zip(*sizes)]
-        numbers = ctypes.c_int32 * pairs
-        self._check(self.lib.fllm_copy_pages((ctypes.c_void_p * len(stores))(*[_ptr(t) for t in stores]), *counts, len(stores), numbers(*source),
-                                             numbers(*target), pairs, self._stream()))
+        i64, i32 = ctypes.c_int64 * count, ctypes.c_int32 * pairs
+        counts = [i64(*column) for column in zip(*sizes)]
+        self._check(self.lib.fllm_copy_pages((ctypes.c_void_p * count)(*addresses), *counts, count, i32(*source), i32(*target), pairs, stream))
 
     # ---- attention over cached latents ------------------------------------------------------------------------------------
     def latent_rope_store(self, joint: torch.Tensor, dkv_at: int, rank: int, rot: int, c_weight: torch.Tensor, eps: float, heads: int, dim: int,
