@@ -626,31 +626,31 @@ int launch_rows(const TreeArgs &a, int max_context, hipStream_t stream) {
     using two = std::integral_constant<int, 2>;
     using four = std::integral_constant<int, 4>;
     using eight = std::integral_constant<int, 8>;
-    // Tiles of 16 rows while every one of them has a compute unit and the keys that they read again are few: a tile's fixed cost (its waves meet
-    // in LDS) goes with its rows.  Microseconds in tiles of 16 / of 32 at 32 heads on 8: a request of 8 nodes at 250, 1,000, 4,000 kept tokens
-    // 7.3 / 9.5, 9.8 / 11.9, 12.4 / 16.4, of 26 nodes at 1,000, 4,000, 8,000 10.4 / 12.2, 13.6 / 14.5, 19.2 / 18.5; 8 of 16 at 1,000 and 4,000
-    // 11.4 / 13.7 and 27.5 / 26.1.
+    // Which tiles.  All figures in microseconds, with keys and values in memory and in no cache, as a step's layers find them.
+    // Of 16 rows while every tile has a compute unit and the keys that the tiles read again are few: a tile's fixed cost (its waves meet in LDS)
+    // goes with its rows.  Tiles of 16 / of 32 at 32 heads on 8: a request of 8 nodes at 250, 1,000, 8,000 kept tokens 7.3 / 9.7, 10.8 / 16.2,
+    // 19.3 / 20.5, of 26 nodes at 2,000 and 4,000 11.9 / 13.7 and 18.2 / 17.5; 8 requests of 8 at 1,000 and 2,000 15.5 / 17.8 and 21.0 / 18.8.
     const long pairs = (long)a.num_segs * a.kv_heads;
     const auto tiles_of = [&](int height) { return height < G ? LONG_MAX / 4 : pairs * ((a.max_nodes + height / G - 1) / (height / G)); };
     const long reach = reach_of(a, max_context);
-    const bool cold = pairs * reach * D * 2 * (long)sizeof(T) > (256l << 20);        // more than the last cache holds
     const int asked = fllm_option_tree_rows();
     const long tiles16 = tiles_of(16);
-    if (G <= 16 && (asked ? asked == 16 : rows <= 16 || (tiles16 <= compute_units() && !cold && (sizeof(T) == 4 || tiles16 * reach <= 600000))))
+    if (G <= 16 && (asked ? asked == 16 : rows <= 16 || (tiles16 <= compute_units() && (sizeof(T) == 4 || tiles16 * reach <= 200000))))
         return go(one(), one(), eight());
     if constexpr (sizeof(T) == 4) {
         return go(two(), one(), eight());
     } else {
-        // Tiles of 32 rows while they fit the device side by side, of 64 where there are more of them.  Heads of 128 go to the kernel whose
-        // rows share every key through LDS where there are more tiles than that, or where the keys and values of all requests are more than
-        // the last cache holds (256 MB): tiles that read them again then read memory again.  Microseconds at 32 heads on 8, tiles of 32 / of 64 /
-        // shared: 8 requests of up to 26 nodes (256 tiles of 32) at 1,000, 4,000, 16,000 kept tokens (393 MB) 12.9 / 18.3 / 24.0,
-        // 30.0 / 33.3 / 39.1, 146 / 152 / 109; of up to 64 nodes (512) at 1,000, 4,000, 16,000 23.9 / 19.2 / 29.2, 48.7 / 45.3 / 54.1,
-        // 223 / 227 / 169; 32 requests of up to 64 nodes at 1,000 84.7 / 61.3 / 47.1.  Heads of 64, tiles of 32 / of 64: 8 requests of up to 26
-        // nodes at 1,000 and 8,000 9.2 / 13.5 and 28.8 / 32.1, of up to 64 nodes 16.4 / 13.9 and 48.7 / 46.5.
-        if (G <= 32 && (asked ? asked <= 32 : rows <= 32 || (tiles_of(32) <= compute_units() && !cold))) return go(two(), one(), eight());
+        // Of 32 rows while they fit the device side by side, of 64 where there are more of them.  Heads of 128 go to the kernel whose rows share
+        // every key through LDS where there are more tiles than that, or where much is read again.  Tiles of 32 / of 64 / shared: 8 requests
+        // of up to 26 nodes (256 tiles of 32) at 1,000, 4,000, 8,000 kept tokens 17.7 / 22.3 / 25.8, 43.9 / 48.7 / 46.6, 78.5 / 82.5 / 70.8; of up
+        // to 64 nodes (512) 29.3 / 23.9 / 30.9, 67.9 / 64.9 / 63.5, 121 / 119 / 103; 32 of up to 26 (1,024) at 1,000 60.6 / 46.5 / 43.1.
+        // Heads of 64, tiles of 32 / of 64: 8 of up to 26 nodes at 1,000, 4,000, 8,000 11.7 / 14.9, 25.6 / 24.7, 43.2 / 38.1; 32 of up to 26 at
+        // 1,000 39.3 / 29.3.
+        const long tiles32 = tiles_of(32);
+        const bool much = tiles32 * (double)reach > (D == 128 ? 1500000 : 900000);
+        if (G <= 32 && (asked ? asked <= 32 : rows <= 32 || (tiles32 <= compute_units() && !much))) return go(two(), one(), eight());
         if constexpr (D == 64) return go(four(), one(), eight());
-        else if (asked ? asked == 128 : cold || tiles_of(64) > 2 * compute_units()) return fllm_tree_attention_wide(a, max_context, stream);
+        else if (asked ? asked == 128 : much || tiles_of(64) >= 2 * compute_units()) return fllm_tree_attention_wide(a, max_context, stream);
         else return go(two(), two(), four());
     }
 }
