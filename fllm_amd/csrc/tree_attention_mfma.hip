@@ -1,15 +1,21 @@
 // Attention of trees of drafted tokens on the matrix cores, bfloat16 and float32: scores, softmax statistics and outputs accumulate in
 // float32.
 //
-// A workgroup of four waves takes a tile of 16 NT rows (nodes x the query heads of one key/value head) and a stretch of the request's slots;
-// the waves take blocks of neighbouring slots in turn, each with a running maximum and sum a row, and meet in LDS at the end.  Keys and
-// values go from the pages straight into matrix operands, the next block's on their way while a block is multiplied:
+// A workgroup of eight waves takes a tile of 16 to 64 rows (nodes x the query heads of one key/value head) and a stretch of the request's
+// slots; the waves (or pairs of them, where each has half of the rows) take blocks of neighbouring slots in turn, each with a running
+// maximum and sum a row, and meet in LDS at the end.  Keys and values go from the pages straight into matrix operands, the next block's
+// on their way while a block is multiplied:
 //   S^T[key][row] = K[key][:] . Q[row][:]          O^T[d][row] += V^T[d][key] P^T[key][row]
 // so that a lane keeps one row (of every 16) throughout and probabilities never leave its registers.
-//   bfloat16  v_mfma_f32_16x16x32: blocks of 64 slots; a lane (c, g) of a score tile has the slots 4 g + i of row c and wants 8 g .. 8 g + 7,
-//             so rows of 16 lanes change places between two tiles and a value load is 16 bytes, 8 neighbouring tokens.
-//   float32   v_mfma_f32_16x16x4: blocks of 32 slots; product e of four takes lane d = 16 j + 4 g + e of keys and queries, product i of four
+//   bfloat16  v_mfma_f32_16x16x32: blocks of 32 slots; a lane (c, g) has the scores of row c and wants those of slots 8 g .. 8 g + 7, so that a
+//             value load is 16 bytes, 8 neighbouring tokens.
+//   float32   v_mfma_f32_16x16x4: blocks of 16 slots; product e of four takes lane d = 16 j + 4 g + e of keys and queries, product i of four
 //             the slots 4 g + i: the operands are the elements of 16-byte loads, and the scores are the second product's operand as they are.
+// What bounds it, with keys and values in memory: few tiles, the trips to memory that follow each other (a request of 8 nodes at 1,000
+// tokens of the 8B sizes 10.2 us, of which an empty launch is 2 and the parts' meeting 3); tiles as many as compute units, what a unit
+// gets from L2 (8 requests of up to 26 nodes at 2,048: four tiles read every key, 27 us, 8.5 TB/s of them); full tiles of heads of 64, the
+// exponentials and the other vector instructions (32 requests of up to 64 nodes at 6,144 149 us; with all keys in L2 123); float32, the
+// matrix cores.  Blocks of twice the slots, or keys asked for two blocks ahead, need registers that two waves a SIMD do not have.
 // Slots that every row of the tile sees need no mask; a block that holds nodes, the end, the window's edge or a page that is none gets a
 // 64-bit mask a row.
 #include "common.h"
@@ -19,7 +25,6 @@
 int fllm_tree_attention_wide(const TreeArgs &a, int max_context, hipStream_t stream);      // tree_attention_wide.hip
 
 namespace {
-
 
 template <typename T> struct Operand;
 template <> struct Operand<bf16_t> {
@@ -48,15 +53,9 @@ __device__ __forceinline__ bf16x8_t neighbours(bf16x8_t p) {
 
 constexpr int q_pitch(int D, bool wide) { return D + (wide ? 4 : 8); }      // elements of a query row in LDS
 
-// The waves are RG groups of rows times KW groups of slots.  Outputs of all slots' groups lie in LDS at a time, or those of half of them, which
-// the other half then adds to its own.
-template <int D, int ROWS, int KW>
-constexpr int groups_together() {
-    return (size_t)KW * ROWS * (D + 4) * sizeof(float) > 140 * 1024 ? KW / 2 : KW;
-}
 template <typename T, int D, int ROWS, int KW>
-constexpr size_t lds_area() {      // the queries while there are slots, the outputs afterwards
-    const size_t queries = (size_t)ROWS * q_pitch(D, sizeof(T) == 4) * sizeof(T), outputs = (size_t)groups_together<D, ROWS, KW>() * ROWS * (D + 4) * sizeof(float);
+constexpr size_t lds_area() {      // the queries while there are slots, the waves' outputs afterwards
+    const size_t queries = (size_t)ROWS * q_pitch(D, sizeof(T) == 4) * sizeof(T), outputs = (size_t)KW * ROWS * (D + 4) * sizeof(float);
     return queries > outputs ? queries : outputs;
 }
 template <typename T, int D, int ROWS, int KW>
@@ -64,19 +63,20 @@ constexpr size_t lds_bytes() {
     return lds_area<T, D, ROWS, KW>() + (size_t)KW * ROWS * 2 * sizeof(float);
 }
 
-// H: value loads of all lanes a block, 32 slots (float32: 16) each.
-// PSH: pages of 1 << PSH tokens; of 8, two a score tile, otherwise of 16, 32 or 64.
+// The waves are RG groups of rows (16 NT each) times KW groups of slots.  PSH: pages of 1 << PSH tokens; of 8, two a score tile, otherwise of
+// 16, 32 or 64.
 // ALONE: no other tile reads the same keys.
-template <typename T, int D, int NT, int PSH, int H, int RG, int KW, int EU, bool ALONE>
-__global__ void __launch_bounds__(RG * KW * kWave) __attribute__((amdgpu_waves_per_eu(EU, EU)))
+template <typename T, int D, int NT, int PSH, int RG, int KW, bool ALONE>
+__global__ void __launch_bounds__(RG * KW * kWave) __attribute__((amdgpu_waves_per_eu(2, 2)))
 tree_attention_kernel(TreeArgs p, TreeSplit sp) {
     typedef typename Operand<T>::vec vec;
     constexpr bool kHalf = sizeof(T) == 2;
+    constexpr int H = 1;                    // value loads of all lanes a block
     constexpr int PER = Operand<T>::kPer, KB = Operand<T>::kStep * H, TILES = KB / 16, THREADS = RG * KW * kWave;
     constexpr int KD = D / (4 * PER);       // 16-byte loads of a key a lane
     constexpr bool P8 = PSH == 3;
     constexpr int PS = 1 << PSH, PMASK = PS - 1;
-    constexpr int DT = D / 16, NP = P8 ? 2 * TILES : TILES, ROWS = 16 * NT * RG, WT = groups_together<D, ROWS, KW>(), QP = q_pitch(D, !kHalf), OP = D + 4;
+    constexpr int DT = D / 16, NP = P8 ? 2 * TILES : TILES, ROWS = 16 * NT * RG, QP = q_pitch(D, !kHalf), OP = D + 4;
     typedef const __attribute__((address_space(4))) int32_t *constant_t;      // the same for every lane: a scalar load
     // what a full exponent adds up to, in the halves of a word or in all of it
     constexpr unsigned kExponents = kHalf ? 0x7f807f80u : 0x7f800000u, kExponentStep = kHalf ? 0x00800080u : 0x00800000u,
@@ -85,7 +85,7 @@ tree_attention_kernel(TreeArgs p, TreeSplit sp) {
     __shared__ int s_row[ROWS], s_lo[ROWS];      // a row's number (-1: none) and the first position it sees
     __shared__ int s_odd;      // a block held values that are not finite and had to be cleared
     T *qs = (T *)lds;                                                     // [ROWS][QP]
-    float *sm_o = (float *)lds;                                           // [WT][ROWS][OP], when the queries have served
+    float *sm_o = (float *)lds;                                           // [KW][ROWS][OP], when the queries have served
     float *sm_m = (float *)(lds + lds_area<T, D, ROWS, KW>()), *sm_l = sm_m + KW * ROWS;
 
     // One grid dimension: the tiles of one (request, part, key/value head) lie on one die, one after the other, so that what the first
@@ -437,16 +437,16 @@ tree_attention_kernel(TreeArgs p, TreeSplit sp) {
         pg = block_pages(kb + KW * KB);
         const int whole_end = min(kept, end) - KB;
         do {
-        while (kb >= lo_max && kb <= whole_end && bad == 0) block(std::true_type());      // slots that every row sees
-        if (kb >= end) break;
-        block(std::false_type());
+            while (kb >= lo_max && kb <= whole_end && bad == 0) block(std::true_type());      // slots that every row sees
+            if (kb >= end) break;
+            block(std::false_type());
         } while (kb < end);
     }
 
     // The groups saw different slots: their statistics and outputs meet, four neighbouring outputs a thread.
     __syncthreads();      // the queries have been read
     const int met = max(1, min(KW, (end - begin + KB - 1) / KB));        // groups that had slots
-    auto put_outputs = [&](int at) {
+    auto put_outputs = [&]() {
 #pragma unroll
         for (int t = 0; t < NT; t++) {
             if (g == 0) {
@@ -454,7 +454,7 @@ tree_attention_kernel(TreeArgs p, TreeSplit sp) {
                 sm_l[kw * ROWS + at_row + t * 16] = l_run[t];
             }
 #pragma unroll
-            for (int dt = 0; dt < DT; dt++) *(f32x4_t *)(sm_o + (at * ROWS + at_row + t * 16) * OP + dt * 16 + 4 * g) = o[t][dt];
+            for (int dt = 0; dt < DT; dt++) *(f32x4_t *)(sm_o + (kw * ROWS + at_row + t * 16) * OP + dt * 16 + 4 * g) = o[t][dt];
         }
     };
 #pragma unroll
@@ -462,28 +462,8 @@ tree_attention_kernel(TreeArgs p, TreeSplit sp) {
         l_run[t] = sum_32_apart(sum_16_apart(l_run[t]));
         m_run[t] = m_run[t] == kNothing ? -INFINITY : m_run[t] * sc;      // in the exponent's units from here on
     }
-    if constexpr (WT < KW) {      // half of the groups at a time, for want of room
-        if (kw >= WT && kw < met) put_outputs(kw - WT);
-        __syncthreads();
-        if (kw + WT < met) {
-#pragma unroll
-            for (int t = 0; t < NT; t++) {
-                const float m1 = sm_m[(kw + WT) * ROWS + at_row + t * 16], m = fmaxf(m_run[t], m1);
-                const float f0 = m_run[t] == -INFINITY ? 0.f : exp2_fast(m_run[t] - m), f1 = m1 == -INFINITY ? 0.f : exp2_fast(m1 - m);
-                m_run[t] = m;
-                l_run[t] = l_run[t] * f0 + sm_l[(kw + WT) * ROWS + at_row + t * 16] * f1;
-#pragma unroll
-                for (int dt = 0; dt < DT; dt++)
-                    o[t][dt] = o[t][dt] * f0 + *(const f32x4_t *)(sm_o + (kw * ROWS + at_row + t * 16) * OP + dt * 16 + 4 * g) * f1;
-            }
-        }
-        __syncthreads();
-        if (kw < min(WT, met)) put_outputs(kw);
-    } else if (kw < met) {
-        put_outputs(kw);
-    }
+    if (kw < met) put_outputs();
     __syncthreads();
-    const int parts_here = min(WT, met);
     const int live_rows = ntok * G;
     const size_t group = ((size_t)seg * p.kv_heads + kvh) * sp.tiles + tile;
     constexpr int PART = ROWS * (D + 4);      // floats of a part: outputs, then a maximum and a sum a row (four words a row)
@@ -502,10 +482,10 @@ tree_attention_kernel(TreeArgs p, TreeSplit sp) {
     for (int idx = threadIdx.x; idx < live_rows * (D / 4); idx += THREADS) {
         const int r = idx / (D / 4), d = (idx - r * (D / 4)) * 4;
         float m = -INFINITY;
-        for (int w = 0; w < parts_here; w++) m = fmaxf(m, sm_m[w * ROWS + r]);
+        for (int w = 0; w < met; w++) m = fmaxf(m, sm_m[w * ROWS + r]);
         float l = 0.f;
         f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
-        for (int w = 0; w < parts_here; w++) {
+        for (int w = 0; w < met; w++) {
             const float mw = sm_m[w * ROWS + r], f = mw == -INFINITY ? 0.f : exp2_fast(mw - m);
             l += sm_l[w * ROWS + r] * f;
             acc += *(const f32x4_t *)(sm_o + (w * ROWS + r) * OP + d) * f;
@@ -580,26 +560,26 @@ tree_attention_kernel(TreeArgs p, TreeSplit sp) {
     }
 }
 
-template <typename T, int D, int NT, int PSH, int H, int RG, int KW, int EU, bool ALONE>
+template <typename T, int D, int NT, int PSH, int RG, int KW, bool ALONE>
 int launch(const TreeArgs &a, int max_context, hipStream_t stream) {
-    constexpr int W = RG * KW, ROWS = 16 * NT * RG;
+    constexpr int ROWS = 16 * NT * RG;
     constexpr size_t smem = lds_bytes<T, D, ROWS, KW>();
     static_assert(smem + 8 * ROWS + 16 <= 160 * 1024, "more than a compute unit's LDS");
     const int G = a.heads / a.kv_heads, TQ = ROWS / G;
     TreeSplit sp;
     sp.tiles = (a.max_nodes + TQ - 1) / TQ;
-    constexpr int round = KW * H * Operand<T>::kStep;
+    constexpr int round = KW * Operand<T>::kStep;
     constexpr size_t part_bytes = (size_t)ROWS * (D + 4) * sizeof(float);
-    plan_tree(a, sp.tiles, compute_units() * (int)std::min((size_t)(4 * EU / W), (160 * 1024) / smem), round, sizeof(T) == 4 ? 1 : 4, max_context, part_bytes, &sp);
+    plan_tree(a, sp.tiles, compute_units(), round, sizeof(T) == 4 ? 1 : 2, max_context, part_bytes, &sp);
     const long units = (long)a.num_segs * sp.splits * a.kv_heads, blocks = (units + 7) / 8 * 8 * sp.tiles;
     FLLM_REQUIRE(blocks <= 0x7fffffffL, "tree_attention: grid too large");
     static bool raised = false;      // more than the default 64 KiB of dynamic LDS has to be asked for once
     if (!raised) {
-        const hipError_t e = hipFuncSetAttribute((const void *)tree_attention_kernel<T, D, NT, PSH, H, RG, KW, EU, ALONE>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        const hipError_t e = hipFuncSetAttribute((const void *)tree_attention_kernel<T, D, NT, PSH, RG, KW, ALONE>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         FLLM_REQUIRE(e == hipSuccess, "tree_attention: cannot raise the LDS limit: %s", hipGetErrorString(e));
         raised = true;
     }
-    hipLaunchKernelGGL((tree_attention_kernel<T, D, NT, PSH, H, RG, KW, EU, ALONE>), dim3((unsigned)blocks), dim3(W * kWave), smem, stream, a, sp);
+    hipLaunchKernelGGL((tree_attention_kernel<T, D, NT, PSH, RG, KW, ALONE>), dim3((unsigned)blocks), dim3(RG * KW * kWave), smem, stream, a, sp);
     return fllm_check_launch("tree_attention");
 }
 
@@ -613,9 +593,9 @@ int launch_rows(const TreeArgs &a, int max_context, hipStream_t stream) {
         auto of_page = [&](auto psh) {
             constexpr int PSH = decltype(psh)::value;
             if constexpr (RG == 1 && NT < 4) {
-                if (alone) return launch<T, D, NT, PSH, 1, RG, KW, 2, true>(a, max_context, stream);
+                if (alone) return launch<T, D, NT, PSH, RG, KW, true>(a, max_context, stream);
             }
-            return launch<T, D, NT, PSH, 1, RG, KW, 2, false>(a, max_context, stream);
+            return launch<T, D, NT, PSH, RG, KW, false>(a, max_context, stream);
         };
         if (a.page_size == 8) return of_page(std::integral_constant<int, 3>());
         if (a.page_size == 16) return of_page(std::integral_constant<int, 4>());
