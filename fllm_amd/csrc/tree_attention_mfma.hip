@@ -14,7 +14,7 @@
 // What bounds it, with keys and values in memory: few tiles, the trips to memory that follow each other (a request of 8 nodes at 1,000
 // tokens of the 8B sizes 10.2 us, of which an empty launch is 2 and the parts' meeting 3); tiles as many as compute units, what a unit
 // gets from L2 (8 requests of up to 26 nodes at 2,048: four tiles read every key, 27 us, 8.5 TB/s of them); full tiles of heads of 64, the
-// exponentials and the other vector instructions (32 requests of up to 64 nodes at 6,144 149 us; with all keys in L2 123); float32, the
+// exponentials and the other vector instructions (32 requests of up to 64 nodes at 6,144 144 us; with all keys in L2 120); float32, the
 // matrix cores.  Blocks of twice the slots, or keys asked for two blocks ahead, need registers that two waves a SIMD do not have.
 // Slots that every row of the tile sees need no mask; a block that holds nodes, the end, the window's edge or a page that is none gets a
 // 64-bit mask a row.
@@ -278,6 +278,15 @@ tree_attention_kernel(TreeArgs p, TreeSplit sp) {
         for (int dt = 0; dt < DT; dt++) load_values(kb, pg, dt);
     }
     __syncthreads();
+    // heads of 64 leave registers for the queries (32 requests of up to 64 nodes at 6,144: 149 -> 144 us); of 128 they stay in LDS
+    constexpr bool kHeld = D == 64;
+    vec qf[kHeld ? NT : 1][KD];
+    if constexpr (kHeld) {
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int j = 0; j < KD; j++) qf[t][j] = *(const vec *)(qs + (at_row + t * 16) * QP + (4 * j + g) * PER);
+    }
     unsigned bad = pg.bad;
     // a block's scores, weights and products; the next block's keys and values are asked for as soon as this one's are used
     auto block = [&](auto whole_block) __attribute__((always_inline)) {
@@ -305,7 +314,9 @@ tree_attention_kernel(TreeArgs p, TreeSplit sp) {
         for (int j = 0; j < KD; j++) {
 #pragma unroll
             for (int t = 0; t < NT; t++) {
-                const vec qv = *(const vec *)(qs + (at_row + t * 16) * QP + (4 * j + g) * PER);
+                vec qv;
+                if constexpr (kHeld) qv = qf[t][j];
+                else qv = *(const vec *)(qs + (at_row + t * 16) * QP + (4 * j + g) * PER);
 #pragma unroll
                 for (int k = 0; k < TILES; k++) {
                     if constexpr (kHalf) {
