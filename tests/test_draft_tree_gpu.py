@@ -343,3 +343,108 @@ def test_refusals(ops):
                                          ((k,) * 9, [0], [1]), ((k.cpu(),), [0], [1]), ((k.transpose(3, 4),), [0], [1]), ((k.view(-1),), [0], [1])):
         with pytest.raises(KernelError):
             ops.copy_pages(stores_given, source, target)
+
+
+# ---- together, captured, and in a large cache -------------------------------------------------------------------------------
+@pytest.mark.parametrize("dim", [64, 128])
+def test_a_captured_run_of_all(ops, dim):
+    """Attention over a split context, the walk and the move in one graph, replayed with other inputs and with eager calls (other sizes, the same
+    workspace) between the replays; a second graph shares the workspace with it."""
+    cases = [plain.TreeCase([(2500, 20), (900, 7)], 8, 2, dim, 16, torch.bfloat16, seed=s) for s in range(3)]
+    other = plain.TreeCase([(3300, 9)], 8, 2, dim, 16, torch.bfloat16, seed=9)
+    rng = random.Random(dim)
+    walks = []
+    for case in cases:
+        drafted, picks, want = [], [], []
+        for parents in case.parents:
+            tokens, mine = [rng.randrange(4) for _ in parents], [rng.randrange(4) for _ in parents]
+            want.append(plain.follow(parents, tokens, mine, 6))
+            drafted += tokens
+            picks += mine
+        walks.append((drafted, picks, want))
+    dev = lambda t: t.clone().cuda()
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    static = dict(q=dev(cases[0].joint[:, : 8 * dim]), k=dev(cases[0].k_pages)[None], v=dev(cases[0].v_pages)[None], tables=dev(cases[0].tables),
+                  pos=dev(cases[0].row_pos), seen=dev(cases[0].seen), parents=i32([p for t in cases[0].parents for p in t]), drafted=i32(walks[0][0]), chosen=i32(walks[0][1]))
+    starts, kept = dev(cases[0].seg_start), dev(cases[0].kept)
+    out = torch.zeros((27, 8 * dim), dtype=torch.bfloat16, device="cuda")
+    path, length, newest = i32([[0] * 6] * 2), i32([0, 0]), i32([0, 0])
+
+    def run():
+        ops.tree_attention(static["q"], static["k"][0], static["v"][0], static["tables"], static["pos"], starts, kept, static["seen"], out, 8, 2, dim, 16, dim ** -0.5, 2520)
+        ops.follow_tree(static["drafted"], static["parents"], starts, static["chosen"], path, length, newest)
+        ops.move_tokens(static["k"], static["v"], static["tables"], kept, path, length)
+
+    graphs = []
+    run()
+    torch.cuda.synchronize()
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            run()
+        graphs.append(graph)
+    for turn in range(6):
+        case, (drafted, picks, want) = cases[turn % 3], walks[turn % 3]
+        static["q"].copy_(case.joint[:, : 8 * dim]), static["k"][0].copy_(case.k_pages), static["v"][0].copy_(case.v_pages), static["tables"].copy_(case.tables)
+        static["pos"].copy_(case.row_pos), static["seen"].copy_(case.seen), static["parents"].copy_(i32([p for t in case.parents for p in t]))
+        static["drafted"].copy_(i32(drafted)), static["chosen"].copy_(i32(picks))
+        check(ops, other)                                   # eager work in the same workspace
+        graphs[turn % 2].replay()
+        torch.cuda.synchronize()
+        expected, bound = case.expected(dim ** -0.5)
+        assert plain.compare(out, expected, bound) <= 1.0
+        assert length.tolist() == [len(p) for p, _ in want] and newest.tolist() == [t for _, t in want]
+        for s, (steps, _) in enumerate(want):               # what the walk kept lies behind the kept tokens
+            for i, node in enumerate(steps):
+                slot = case.requests[s][0] + i
+                page = int(case.tables[s, slot // 16])
+                assert torch.equal(static["v"][0, page, :, :, slot % 16].cpu(), case.values[s][case.requests[s][0] + node])
+                assert torch.equal(static["k"][0, page, :, :, slot % 16].cpu().reshape(2, dim), case.keys[s][case.requests[s][0] + node])
+
+
+@pytest.mark.parametrize("dtype,dim,rows", [(torch.bfloat16, 128, 16), (torch.bfloat16, 128, 64), (torch.bfloat16, 128, 128), (torch.bfloat16, 64, 64), (torch.float32, 64, 0), (torch.float32, 40, 0)])
+def test_offsets_beyond_32_bits(ops, dtype, dim, rows):
+    """The last pages of a cache of more than 2^32 bytes, and a second layer behind it."""
+    case = plain.TreeCase([(150, 20), (33, 5)], 8, 8, dim, 16, dtype, seed=dim + rows)
+    small = case.k_pages.shape[0]
+    pages = -(-(1 << 31) // (8 * dim * 16)) + 5 + small            # more than 2^31 elements of keys, and as many values
+    k = torch.empty((2, pages, 8, dim // 8, 16, 8), dtype=dtype, device="cuda")
+    v = torch.empty((2, pages, 8, dim, 16), dtype=dtype, device="cuda")
+    first = pages - small
+    for layer in range(2):
+        k[layer, first:], v[layer, first:] = case.k_pages.cuda(), case.v_pages.cuda()
+    tables = torch.where(case.tables >= 0, case.tables + first, case.tables).cuda()
+    want, bound = case.expected(0.1)
+    ops.set_option("attention.tree_rows", rows)
+    try:
+        for layer in range(2):
+            out = torch.zeros((case.rows, 8 * dim), dtype=dtype, device="cuda")
+            ops.tree_attention(case.joint[:, : 8 * dim].cuda(), k[layer], v[layer], tables, case.row_pos.cuda(), case.seg_start.cuda(), case.kept.cuda(), case.seen.cuda(), out, 8, 8, dim, 16,
+                               0.1, 170)
+            assert plain.compare(out, want, bound) <= 1.0
+    finally:
+        ops.set_option("attention.tree_rows", 0)
+    path, length = torch.tensor([[0, 3, 19], [0, 4, -1]], dtype=torch.int32, device="cuda"), torch.tensor([3, 2], dtype=torch.int32, device="cuda")
+    ops.move_tokens(k, v, tables, case.kept.cuda(), path, length)
+    for s, i, node in ((0, 1, 3), (0, 2, 19), (1, 1, 4)):
+        slot = case.requests[s][0] + i
+        page = int(tables[s, slot // 16])
+        for layer in range(2):
+            assert torch.equal(v[layer, page, :, :, slot % 16].cpu(), case.values[s][case.requests[s][0] + node])
+            assert torch.equal(k[layer, page, :, :, slot % 16].cpu().reshape(8, dim), case.keys[s][case.requests[s][0] + node])
+    k[1, pages - 1], v[1, pages - 1] = 3.0, 4.0
+    ops.copy_pages((k, v), [pages - 1], [first - 1])
+    assert bool((k[1, first - 1] == 3.0).all()) and bool((v[1, first - 1] == 4.0).all())
+
+
+def test_another_stream_is_refused(ops):
+    """As for every kernel that meets others in the device workspace."""
+    from fllm_amd.kernels import KernelError
+    case = plain.TreeCase([(20, 4)], 4, 2, 64, 16, torch.bfloat16, seed=1)
+    check(ops, case)
+    with torch.cuda.stream(torch.cuda.Stream()):
+        with pytest.raises(KernelError, match="stream"):
+            attend(ops, case, 0.1)
+        with pytest.raises(KernelError, match="stream"):
+            ops.copy_pages((torch.zeros((1, 4, 8), device="cuda"),), [0], [1])
+    torch.cuda.synchronize()
