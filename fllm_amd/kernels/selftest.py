@@ -8,7 +8,7 @@ from typing import Callable, Dict, List, Optional
 
 import torch
 
-GROUPS = ["embedding", "norm", "linear", "fused", "activation", "rope_kv", "attention", "sampling"]
+GROUPS = ["embedding", "norm", "linear", "fused", "activation", "rope_kv", "attention", "drafts", "sampling"]
 
 
 def _err(got: torch.Tensor, want: torch.Tensor) -> float:
@@ -128,6 +128,44 @@ def _attention(ops, dev, report):
             report(f"attention {dtype} {segs} window={window}", _err(got, want.view(rows, -1)), tol)
 
 
+def _drafts(ops, dev, report):
+    """Trees of drafted tokens: their attention, the walk along the model's choices, kept tokens moved up, copied pages."""
+    from . import tree_rows
+    heads, kv_heads, ps, parents = 8, 2, 16, [-1, 0, 0, 1, 1, 2, 3, 3, 6]
+    nodes = len(parents)
+    for dtype, d, kept, tol in ((torch.float32, 64, 300, 2e-6), (torch.bfloat16, 64, 300, 2 ** -6), (torch.bfloat16, 128, 4000, 2 ** -6), (torch.bfloat16, 40, 70, 2 ** -6)):
+        pages = -(-(kept + nodes) // ps)
+        tables = torch.randperm(pages, device=dev).to(torch.int32)[None]
+        k, v = torch.randn(2, pages, kv_heads, d // 8, ps, 8, device=dev).to(dtype), torch.randn(2, pages, kv_heads, d, ps, device=dev).to(dtype)
+        i32 = lambda values: torch.tensor(values, dtype=torch.int32, device=dev)
+        depths, seen = tree_rows(parents)
+        q = torch.randn(nodes, heads * d, device=dev).to(dtype)
+        got = ops.tree_attention(q, k[0], v[0], tables, i32([kept + n for n in depths]), i32([0, nodes]), i32([kept]), torch.tensor(seen, dtype=torch.int64, device=dev),
+                                 torch.empty(nodes, heads * d, dtype=dtype, device=dev), heads, kv_heads, d, ps, d ** -0.5, kept + nodes)
+        slot = torch.arange(kept + nodes, device=dev)
+        pg, off = tables[0, (slot // ps).long()].long(), (slot % ps).long()
+        kk = k[0][pg, :, :, off, :].double().reshape(-1, kv_heads, d).repeat_interleave(heads // kv_heads, 1).permute(1, 2, 0).contiguous()
+        vv = v[0][pg, :, :, off].double().repeat_interleave(heads // kv_heads, 1).permute(1, 0, 2).contiguous()
+        z = torch.bmm(q.double().view(nodes, heads, d).permute(1, 0, 2).contiguous(), kk) * d ** -0.5
+        hidden = torch.tensor([[j < kept or bool(seen[i][0] >> (j - kept) & 1) for j in range(kept + nodes)] for i in range(nodes)], device=dev).logical_not()
+        want = torch.bmm(torch.softmax(z.masked_fill(hidden, -math.inf), -1), vv).permute(1, 0, 2).reshape(nodes, -1)
+        report(f"tree_attention {dtype} heads of {d} at {kept}", _err(got, want), tol)
+        path, length, newest = i32([[0] * 5]), i32([0]), i32([0])
+        ops.follow_tree(i32(range(nodes)), i32(parents), i32([0, nodes]), i32([1, 3, 5, 6, 0, 0, 0, 0, 0]), path, length, newest)
+        ok = path.tolist() == [[0, 1, 3, 6, -1]] and length.tolist() == [4] and newest.tolist() == [0]
+        report("follow_tree", 0.0 if ok else 1.0, 0.0)
+        wants = [t.clone() for t in (k, v)]
+        for want, t in zip(wants, (k, v)):
+            for i, node in ((2, 3), (3, 6)):
+                (to, b), (at, a) = divmod(kept + i, ps), divmod(kept + node, ps)
+                want[:, int(tables[0, to]), :, :, b] = t[:, int(tables[0, at]), :, :, a]
+        ops.move_tokens(k, v, tables, i32([kept]), path, length)
+        ops.copy_pages((k, v), [0, 0], [1, pages - 1])
+        for want in wants:
+            want[:, [1, pages - 1]] = want[:, :1]
+        report(f"move_tokens and copy_pages {dtype}", max(_err(a, b) for a, b in zip((k, v), wants)), 0.0)
+
+
 def _sampling(ops, dev, report):
     logits = torch.randn(5, 1000, device=dev)
     logits[0, 7] = logits[0, 900] = 60.0
@@ -137,7 +175,7 @@ def _sampling(ops, dev, report):
 
 
 _CHECKS: Dict[str, Callable] = {"embedding": _embedding, "norm": _norm, "linear": _linear, "fused": _fused, "activation": _activation,
-                                "rope_kv": _rope_kv, "attention": _attention, "sampling": _sampling}
+                                "rope_kv": _rope_kv, "attention": _attention, "drafts": _drafts, "sampling": _sampling}
 
 
 def run(only: Optional[List[str]] = None, device: str = "cuda:0") -> int:

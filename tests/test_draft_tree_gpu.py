@@ -271,6 +271,17 @@ def test_copying(ops, pairs, shapes, dtype):
         assert torch.equal(a, b.cpu())
 
 
+def test_copying_more_pages_than_a_launch_takes(ops):
+    rng = random.Random(7)
+    chosen = rng.sample(range(2000), 1300)
+    source, target = chosen[:30] * 33, chosen[310:1300]
+    store = torch.randn((2, 2000, 3, 8), generator=torch.Generator().manual_seed(1))
+    device = store.cuda()
+    ops.copy_pages((device,), source, target)
+    store[:, target] = store[:, source]
+    assert torch.equal(device.cpu(), store)
+
+
 def test_rotary_positions_that_are_not_slots(ops):
     """`rope_kv_store(row_slot=)` stores at the slot what the call without it stores at the position."""
     from fllm_amd.kernels import KernelError
