@@ -39,7 +39,8 @@ __device__ __forceinline__ bf16x8_t pack8(const f32x4_t &lo, const f32x4_t &hi) 
     return p;
 }
 
-constexpr float kNothing = -3e38f;      // the reference point of a row that has seen nothing: below every score, and still finite
+// The reference point of a row that has seen nothing: below every score, and still finite, in the exponent's units (of scales above 1) too.
+constexpr float kNothing = -3e38f;
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // the `count` lowest bits

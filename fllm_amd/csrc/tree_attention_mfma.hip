@@ -235,16 +235,16 @@ tree_attention_kernel(TreeArgs p, TreeSplit sp) {
         return s_row[at_row + t * 16] < 0 ? 0ull : bits;
     };
 
+    const float sc = sp.scale, tau = 8.0f / sc, nothing = kNothing / fmaxf(sc, 1.0f);
     f32x4_t o[NT][DT];
     float m_run[NT], l_run[NT];      // the reference point in raw units; the sum over the lane's own slots
 #pragma unroll
     for (int t = 0; t < NT; t++) {
-        m_run[t] = kNothing;
+        m_run[t] = nothing;
         l_run[t] = 0.f;
 #pragma unroll
         for (int dt = 0; dt < DT; dt++) o[t][dt] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
     }
-    const float sc = sp.scale, tau = 8.0f / sc;
 
     int kb = begin + kw * KB;
     Pages pg = block_pages(kb);
@@ -369,7 +369,7 @@ tree_attention_kernel(TreeArgs p, TreeSplit sp) {
         vec pv[NT][H];        // the weights as the second product takes them
 #pragma unroll
         for (int t = 0; t < NT; t++) {
-            const float mc = WHOLE ? m_run[t] * sc : fmaxf(m_run[t] * sc, kNothing);      // finite for a row that has seen nothing
+            const float mc = m_run[t] * sc;      // finite for a row that has seen nothing
             float sum = 0.f;
 #pragma unroll
             for (int k = 0; k < TILES; k++)
@@ -471,7 +471,7 @@ tree_attention_kernel(TreeArgs p, TreeSplit sp) {
 #pragma unroll
     for (int t = 0; t < NT; t++) {
         l_run[t] = sum_32_apart(sum_16_apart(l_run[t]));
-        m_run[t] = m_run[t] == kNothing ? -INFINITY : m_run[t] * sc;      // in the exponent's units from here on
+        m_run[t] = m_run[t] == nothing ? -INFINITY : m_run[t] * sc;      // in the exponent's units from here on
     }
     if (kw < met) put_outputs();
     __syncthreads();

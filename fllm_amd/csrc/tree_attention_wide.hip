@@ -119,8 +119,8 @@ tree_wide_kernel(TreeArgs p, TreeSplit sp) {
     for (int db = 0; db < DB; db++)
 #pragma unroll
         for (int i = 0; i < 16; i++) o[db][i] = 0.f;
-    float m_run = kNothing, l_run = 0.f;       // the reference point in raw units; the sum over the lane's own slots
-    const float sc = sp.scale, tau = 8.0f / sc;
+    const float sc = sp.scale, tau = 8.0f / sc, nothing = kNothing / fmaxf(sc, 1.0f);
+    float m_run = nothing, l_run = 0.f;       // the reference point in raw units; the sum over the lane's own slots
     if (threadIdx.x == 0) s_odd = 0;
     const int whole_end = min(kept, end) - KT;
 
@@ -233,7 +233,7 @@ tree_wide_kernel(TreeArgs p, TreeSplit sp) {
                 for (int i = 0; i < 16; i++) o[db][i] *= alpha;
             m_run = m_new;
         }
-        const float mc = fmaxf(m_run * sc, kNothing);      // finite for a row that has seen nothing
+        const float mc = m_run * sc;      // finite for a row that has seen nothing
         float sum = 0.f;
 #pragma unroll
         for (int rb = 0; rb < 2; rb++)
@@ -271,7 +271,7 @@ tree_wide_kernel(TreeArgs p, TreeSplit sp) {
                 }
         }
     }
-    float l = sum_32_apart(l_run), m = m_run == kNothing ? -INFINITY : m_run * sc;      // in the exponent's units from here on
+    float l = sum_32_apart(l_run), m = m_run == nothing ? -INFINITY : m_run * sc;      // in the exponent's units from here on
     if (live > 1) {
         // A part leaves its outputs, maximum and sum, each lane its own; the part that arrives last adds them up in their order.
         const size_t group = ((size_t)seg * nkv + kvh) * sp.tiles + tile;

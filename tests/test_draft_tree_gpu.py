@@ -459,3 +459,25 @@ def test_another_stream_is_refused(ops):
         with pytest.raises(KernelError, match="stream"):
             ops.copy_pages((torch.zeros((1, 4, 8), device="cuda"),), [0], [1])
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("dim,rows", [(64, 0), (128, 0), (128, 64), (128, 128), (64, 64), (40, 0)])
+@pytest.mark.parametrize("scale", [0.1, 2.0])
+def test_scores_of_minus_infinity(ops, dim, rows, scale, dtype):
+    """Keys that make a score minus infinity weigh nothing: whole blocks of them ahead of, between and behind others, with scales on both sides of 1."""
+    case = plain.TreeCase([(700, 9), (90, 20)], 4, 2, dim, 16 if dim != 40 else 8, dtype, seed=dim)
+    case.joint = case.joint.abs() + 0.1                # times minus infinity: that, in every lane
+    case.joint *= 0.25
+    none = {0: set(range(0, 300)) | set(range(420, 500)) | set(range(650, 700)), 1: set(range(0, 64)) | {92}}
+    visible = case.visible
+    case.visible = lambda s, i, window: [t for t in visible(s, i, window) if t not in none[s]]
+    for s, slots in none.items():
+        for t in slots:
+            case.keys[s][t, :, 3] = float("-inf")
+            case.put(s, t)
+    ops.set_option("attention.tree_rows", rows)
+    try:
+        check(ops, case, scale=scale)
+    finally:
+        ops.set_option("attention.tree_rows", 0)
