@@ -23,6 +23,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 struct TreeSplit {
     int tiles;            // row tiles a request at most
     int splits, per;      // parts of the slots, slots a part (the last takes what is left)
+    int places;           // where the kernel cuts the slots itself: places a die (per: rounds a part at least)
     int *counters;        // one per (request, key/value head, tile), zero between launches
     float *parts;         // [request, key/value head, tile][split][16 NT rows of D outputs, then of a maximum and a sum]
     float scale;          // >= 0: the sign has gone into the queries

@@ -633,8 +633,8 @@ int launch_rows(const TreeArgs &a, int max_context, hipStream_t stream) {
     } else {
         // Of 32 rows while they fit the device side by side, of 64 where there are more of them.  Heads of 128 go to the kernel whose rows share
         // every key through LDS where there are more tiles than that, or where much is read again.  Tiles of 32 / of 64 / shared: 8 requests
-        // of up to 26 nodes (256 tiles of 32) at 1,000, 4,000, 8,000 kept tokens 17.7 / 22.3 / 25.8, 43.9 / 48.7 / 46.6, 78.5 / 82.5 / 70.8; of up
-        // to 64 nodes (512) 29.3 / 23.9 / 30.9, 67.9 / 64.9 / 63.5, 121 / 119 / 103; 32 of up to 26 (1,024) at 1,000 60.6 / 46.5 / 43.1.
+        // of up to 26 nodes (256 tiles of 32) at 1,000, 4,000, 8,000 kept tokens 17.9 / 22.5 / 25.3, 44.1 / 49.4 / 44.7, 78.7 / 83.7 / 65.6; of up
+        // to 64 nodes (512) 29.8 / 24.0 / 30.0, 68.6 / 65.0 / 59.5, 115 / 120 / 92; 32 of up to 26 (1,024) at 1,000 61.7 / 48.1 / 41.4.
         // Heads of 64, tiles of 32 / of 64: 8 of up to 26 nodes at 1,000, 4,000, 8,000 11.7 / 14.9, 25.6 / 24.7, 43.2 / 38.1; 32 of up to 26 at
         // 1,000 39.3 / 29.3.
         const long tiles32 = tiles_of(32);

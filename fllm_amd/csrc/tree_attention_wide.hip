@@ -8,15 +8,134 @@
 // wants: the keys lie in LDS in the order that makes it so (bits 2 and 3 of a slot's number swapped).
 // Masks, what is not finite, and parts that several workgroups make of a tile's slots: as in tree_attention_mfma.hip.
 //
-// Two requests of 64 nodes at 32,768 tokens, 64 heads of 128 on 8: 178 us, 0.56 PFLOP/s, 1.4 TB/s of keys and values in whatever cache they
-// lie (all of them in one page: 161).  Matrix cores, vector instructions and LDS are busy a third of that each, and a wave waits for the one
-// before the other; with two waves a SIMD little of it overlaps.  Two or four tiles on their way instead of one: the same (179, and for four
-// no registers).  Eight waves of 256 rows: 169, and 49 instead of 36 us for one request of 32 nodes at 8,000.  Two blocks of 32 rows a wave,
-// the products of one beside the weights of the other, need more registers than a wave has (279).
+// Two requests of 64 and 34 nodes at 32,768 and 28,593 tokens, 64 heads of 128 on 8: 146 us, 0.69 PFLOP/s.  Bound by the matrix
+// cores' rate on real numbers, 1.7 to 1.95 PFLOP/s (zeros: 2.5), and by what does not fit beside the products: with parts of the loop left out in
+// turn the weights took 28 us, LDS reads 12, stores to LDS 15.  One product behind the other on one sum takes 52 cycles instead of 32: the
+// scores take turns on two.  Operands are read from LDS six products ahead (written as a plain loop each is waited for: 178 us -> 164), the requests' slots are
+// cut by what their lengths are (164 -> 155), the weights of a tile's second half are made between the products of the first, and a wave
+// that multiplies goes ahead of the one that makes weights (153 -> 146; either alone 150 to 153).
+// The same: 4 or 8 products ahead; two teams of waves that take turns at products and weights between barriers (152 to 158); four tiles on
+// their way instead of one has no registers; 64 rows a wave with one wave a SIMD spills (275).
+
 #include "draft_api.h"
 #include "tree_attention.h"
 
 namespace {
+
+struct Place {
+    int seg, unit, tile;      // request (-1: no work), part x key/value head, row tile
+    int parts, per, tiles;    // of the request: parts of its slots, slots a part, tiles
+    int start, turn;          // the request's first place on a die, and the die that its first unit lies on
+    // the workgroup that has a unit of the request, of this tile
+    __device__ __forceinline__ unsigned block_of(int u) const { return (unsigned)((start + u / 8 * tiles + tile) * 8 + (u + turn) % 8); }
+};
+
+// Where a workgroup works.  The requests' lengths are known here and not to the host: all of them are looked over (64 at a time, one a lane) and
+// cut so that the workgroups that the device holds at a time (sp.places on each of 8 dies) have about as much each: parts of at most `per`
+// rounds of KT slots.  The tiles of one (request, part, key/value head) lie on one die, one after the other.  Without places (at least as many
+// requests and key/value heads as workgroups) every request stays whole and nothing is looked over.
+template <int PSH, int KT>
+__device__ __forceinline__ Place find_place(const TreeArgs &p, const TreeSplit &sp, int TQ) {
+    const int lane = threadIdx.x & (kWave - 1), mine = blockIdx.x / 8, die = blockIdx.x % 8;
+    Place at = {-1, 0, 0, 1, 1 << 28, 1, 0, 0};
+    if (sp.places == 0) {
+        const int unit = mine / sp.tiles * 8 + die;
+        at.tile = mine % sp.tiles;
+        at.unit = unit % p.kv_heads;
+        if (unit < p.num_segs * p.kv_heads) at.seg = unit / p.kv_heads;
+        return at;
+    }
+    auto request = [&](int s, int &tiles, int &rounds) {
+        tiles = rounds = 0;
+        if (s >= p.num_segs) return;
+        const int row0 = max(p.seg_start[s], 0), nodes = min(p.seg_start[s + 1], p.rows) - row0;
+        if (nodes <= 0) return;
+        tiles = (min(nodes, p.max_nodes) + TQ - 1) / TQ;
+        long n = min((long)max(p.kept[s], 0) + nodes, min((long)p.table_stride << PSH, (long)INT_MAX - 4096));
+        if (p.window > 0) n = min(n, (long)p.window + nodes + KT);
+        rounds = (int)((n + KT - 1) / KT);
+    };
+    auto over_lanes = [&](auto v) {
+#pragma unroll
+        for (int step = 32; step > 0; step >>= 1) v += __shfl_xor(v, step);
+        return v;
+    };
+    float work = 0.f;
+    int most = 0;
+    for (int s0 = 0; s0 < p.num_segs; s0 += kWave) {
+        int tiles, rounds;
+        request(s0 + lane, tiles, rounds);
+        work += (float)tiles * (float)rounds;
+        most = max(most, rounds);
+    }
+    work = over_lanes(work);
+#pragma unroll
+    for (int step = 32; step > 0; step >>= 1) most = max(most, __shfl_xor(most, step));
+    auto parts_of = [&](int rounds, int per) { return min((rounds + per - 1) / per, kMostSplits); };
+    int per = max(sp.per, (int)fminf(work * (float)p.kv_heads / (float)(sp.places * 8), 1e8f));
+    while (per < most) {
+        int sum = 0;
+        for (int s0 = 0; s0 < p.num_segs; s0 += kWave) {
+            int tiles, rounds;
+            request(s0 + lane, tiles, rounds);
+            sum += parts_of(rounds, per) * p.kv_heads * tiles;
+        }
+        if (over_lanes(sum) <= sp.places * 8) break;
+        per += 1 + per / 32;
+    }
+    int before = 0;
+    for (int s0 = 0; s0 < p.num_segs; s0 += kWave) {
+        int tiles, rounds;
+        request(s0 + lane, tiles, rounds);
+        const int parts = parts_of(rounds, per), places = (parts * p.kv_heads + 7) / 8 * tiles;
+        int upto = places;
+#pragma unroll
+        for (int step = 1; step < kWave; step <<= 1) {
+            const int low = __shfl_up(upto, step);
+            upto += lane >= step ? low : 0;
+        }
+        const unsigned long long here = __ballot(mine < before + upto);
+        if (here != 0) {
+            const int from = __builtin_ctzll(here);
+            at.parts = __builtin_amdgcn_readlane(parts, from);
+            at.tiles = __builtin_amdgcn_readlane(tiles, from);
+            rounds = __builtin_amdgcn_readlane(rounds, from);
+            at.start = before + __builtin_amdgcn_readlane(upto, from) - __builtin_amdgcn_readlane(places, from);
+            at.per = (rounds + at.parts - 1) / at.parts * KT;
+            at.tile = (mine - at.start) % at.tiles;
+            at.turn = (s0 + from) * p.kv_heads % 8;      // so that few key/value heads use all dies
+            at.unit = (mine - at.start) / at.tiles * 8 + (die + 8 - at.turn) % 8;
+            if (at.unit < at.parts * p.kv_heads) at.seg = s0 + from;
+            break;
+        }
+        before += __builtin_amdgcn_readlane(upto, kWave - 1);
+    }
+    return at;
+}
+
+// The host's side: `slots` workgroups at a time, where the parts that they leave have room in the device workspace; parts of `least` rounds at
+// least.  Returns the places that the grid has on each die.
+long plan_places(const TreeArgs &a, int slots, int least, size_t part_bytes, TreeSplit *sp) {
+    sp->negate = a.scale < 0.f;
+    sp->scale = (a.scale < 0.f ? -a.scale : a.scale) * kLog2e;
+    sp->counters = nullptr;
+    sp->parts = nullptr;
+    sp->splits = 1;
+    sp->per = least;
+    sp->places = 0;
+    const long units = (long)a.num_segs * a.kv_heads, rounded = a.kv_heads % 8 ? (long)a.num_segs * sp->tiles : 0;
+    void *ws = nullptr;
+    size_t ws_bytes = 0;
+    if (units < slots && units * sp->tiles * (long)sizeof(int) <= (long)kWorkspaceCounterBytes && fllm_device_workspace(&ws, &ws_bytes) &&
+        ws_bytes > kWorkspaceCounterBytes) {
+        const long room = (long)(std::min(ws_bytes - kWorkspaceCounterBytes, (size_t)0x7fffffff) / (8 * part_bytes)) - rounded;
+        sp->places = (int)std::max(0l, std::min((long)slots / 8, room));
+        sp->counters = (int *)ws;
+        sp->parts = (float *)((unsigned char *)ws + kWorkspaceCounterBytes);
+    }
+    if (sp->places == 0) return (units + 7) / 8 * sp->tiles;
+    return std::max((long)a.num_segs * ((a.kv_heads + 7) / 8) * sp->tiles, sp->places + rounded);
+}
 
 template <int D, int PSH, int W>
 __global__ void __launch_bounds__(W * kWave) __attribute__((amdgpu_waves_per_eu(2, 2)))
@@ -31,11 +150,10 @@ tree_wide_kernel(TreeArgs p, TreeSplit sp) {
     __shared__ __attribute__((aligned(16))) bf16_t Vs[D * VP];
     __shared__ int s_odd, s_seen;
 
-    // the tiles of one (request, part, key/value head) lie on one die, one after the other
     const int G = p.heads / p.kv_heads, TQ = ROWS / G, nkv = p.kv_heads;
-    const int unit = (int)(blockIdx.x / 8 / sp.tiles) * 8 + (int)(blockIdx.x % 8), tile = (int)(blockIdx.x / 8) % sp.tiles;
-    if (unit >= p.num_segs * sp.splits * nkv) return;
-    const int kvh = unit % nkv, split = unit / nkv % sp.splits, seg = unit / nkv / sp.splits;
+    const Place place = find_place<PSH, KT>(p, sp, TQ);
+    if (place.seg < 0) return;
+    const int kvh = place.unit % nkv, split = place.unit / nkv, seg = place.seg, tile = place.tile;
     const int row0 = max(((constant_t)(uintptr_t)p.seg_start)[seg], 0);
     const int nodes = min(((constant_t)(uintptr_t)p.seg_start)[seg + 1], p.rows) - row0;
     const int kept0 = max(((constant_t)(uintptr_t)p.kept)[seg], 0);
@@ -65,9 +183,9 @@ tree_wide_kernel(TreeArgs p, TreeSplit sp) {
         lo_max = __builtin_amdgcn_readfirstlane(lo_max);
     }
     const int first = max(0, min(lo_min, kept)) / KT * KT;
-    const int live = max(1, (int)min((long)sp.splits, ((long)n - first + sp.per - 1) / sp.per));      // parts that hold slots
+    const int live = max(1, (int)min((long)place.parts, ((long)n - first + place.per - 1) / place.per));      // parts that hold slots
     if (split >= live) return;
-    const int begin = first + split * sp.per, end = split == sp.splits - 1 ? n : min(n, begin + sp.per);
+    const int begin = first + split * place.per, end = split == place.parts - 1 ? n : min(n, begin + place.per);
 
     bf16x8_t qf[DS];
 #pragma unroll
@@ -124,17 +242,18 @@ tree_wide_kernel(TreeArgs p, TreeSplit sp) {
     if (threadIdx.x == 0) s_odd = 0;
     const int whole_end = min(kept, end) - KT;
 
-    int here = pages(begin);       // the tile's page numbers, one a lane: asked for a tile ahead of its keys and values
-    if (begin < end) fetch(here);
+    int here = pages(begin), k0 = begin;       // the tile's page numbers, one a lane: asked for a tile ahead of its keys and values
+    fetch(here);
     int then = pages(begin + KT);
-    for (int k0 = begin; k0 < end; k0 += KT) {
-        const unsigned bad = (unsigned)__ballot((unsigned)here >= (unsigned)p.num_pages);
-        const bool whole = k0 >= lo_max && k0 <= whole_end && bad == 0;
-        const bool nodes_here = k0 + KT > kept;
+    constexpr int kAhead = 6;        // operands on their way from LDS: a read takes as long as four products
+    auto step = [&](auto whole_tile) __attribute__((always_inline)) {
+        constexpr bool WHOLE = decltype(whole_tile)::value;
+        const unsigned bad = WHOLE ? 0u : (unsigned)__ballot((unsigned)here >= (unsigned)p.num_pages);
+        const bool nodes_here = !WHOLE && k0 + KT > kept;
         // a tile with nodes: the row's bits and the nodes' positions come while the tile is stored and the scores are made
         unsigned long long word_low = 0, word_high = 0;
         int at = INT_MIN;
-        if (!whole && nodes_here) {
+        if (nodes_here) {
             const int w = max(k0 - kept, 0) >> 6, j = k0 - kept + lane;
             const int64_t *mine = p.seen + (size_t)max(row, 0) * p.words;
             word_low = (unsigned long long)mine[min(w, p.words - 1)];
@@ -142,7 +261,7 @@ tree_wide_kernel(TreeArgs p, TreeSplit sp) {
             if (p.window > 0 && j >= 0 && j < nodes) at = p.row_pos[row0 + j];
         }
         __syncthreads();   // the previous tile has been read
-        if (!whole) {
+        if constexpr (!WHOLE) {
             // Slots that no row sees may hold anything, and weights of zero do not keep a NaN or an infinity out: they are cleared, and so is
             // what is not finite; the rows that see it are given it at the end.
             unsigned odd = 0;
@@ -168,22 +287,27 @@ tree_wide_kernel(TreeArgs p, TreeSplit sp) {
         }
         __syncthreads();
         here = then;
-        if (k0 + KT < end) {      // on its way while this tile is multiplied
-            fetch(here);
-            then = pages(k0 + 2 * KT);
-        }
+        fetch(here);      // on its way while this tile is multiplied; behind the last: page 0, for nobody
+        then = pages(k0 + 2 * KT);
 
         f32x16_t s[2];
 #pragma unroll
-        for (int rb = 0; rb < 2; rb++) {
+        for (int rb = 0; rb < 2; rb++)
 #pragma unroll
             for (int i = 0; i < 16; i++) s[rb][i] = 0.f;
-            const bf16_t *krow = Ks + (rb * 32 + q) * KP + h * 8;
+        bf16x8_t ring[kAhead];
+        auto key = [&](int i) { return *(const bf16x8_t *)(Ks + (i % 2 * 32 + q) * KP + h * 8 + i / 2 * 16); };
+        auto value = [&](int i) { return *(const bf16x8_t *)(Vs + (i % DB * 32 + q) * VP + i / DB * 16 + 8 * h); };
 #pragma unroll
-            for (int ds = 0; ds < DS; ds++)
-                s[rb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8_t *)(krow + ds * 16), qf[ds], s[rb], 0, 0, 0);
+        for (int i = 0; i < kAhead; i++) ring[i] = key(i);
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int i = 0; i < 2 * DS; i++) {
+            __builtin_amdgcn_sched_barrier(0);
+            s[i % 2] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ring[i % kAhead], qf[i / 2], s[i % 2], 0, 0, 0);
+            if (i + kAhead < 2 * DS) ring[i % kAhead] = key(i + kAhead);
         }
-        if (!whole) {
+        if constexpr (!WHOLE) {
             const int to_kept = kept - k0;
             unsigned long long bits = low_bits(to_kept);
             if (p.window > 0) bits &= ~low_bits(lo_row <= k0 ? 0 : min(lo_row - k0, 64));
@@ -218,6 +342,7 @@ tree_wide_kernel(TreeArgs p, TreeSplit sp) {
                 for (int i = 0; i < 16; i++)
                     if (!(bits >> (rb * 32 + 16 * (i >> 3) + (i & 7)) & 1)) s[rb][i] = -INFINITY;
         }
+        __builtin_amdgcn_s_setprio(0);
         float top = -INFINITY;
 #pragma unroll
         for (int rb = 0; rb < 2; rb++)
@@ -233,30 +358,37 @@ tree_wide_kernel(TreeArgs p, TreeSplit sp) {
                 for (int i = 0; i < 16; i++) o[db][i] *= alpha;
             m_run = m_new;
         }
+#pragma unroll
+        for (int i = 0; i < kAhead; i++) ring[i] = value(i);
+        __builtin_amdgcn_sched_barrier(0);
         const float mc = m_run * sc;      // finite for a row that has seen nothing
-        float sum = 0.f;
+        bf16x8_t pf[4];
+        auto weight = [&](int i) {
+            const float w = exp2_fast(fmaf(s[i >> 4][i & 15], sc, -mc));
+            l_run += w;
+            pf[i >> 3][i & 7] = (bf16_t)w;      // a weight is rounded to bfloat16 where it meets the values
+        };
 #pragma unroll
-        for (int rb = 0; rb < 2; rb++)
+        for (int i = 0; i < 16; i++) weight(i);      // those of the second 32 slots beside the products of the first
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
-                s[rb][i] = exp2_fast(fmaf(s[rb][i], sc, -mc));
-                sum += s[rb][i];
+        for (int i = 0; i < 4 * DB; i++) {
+            __builtin_amdgcn_sched_barrier(0);
+            o[i % DB] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ring[i % kAhead], pf[i / DB], o[i % DB], 0, 0, 0);
+            if (i + kAhead < 4 * DB) ring[i % kAhead] = value(i + kAhead);
+            if (i < 2 * DB) {
+#pragma unroll
+                for (int e = 0; e < 8 / DB; e++) weight(16 + i * (8 / DB) + e);
             }
-        l_run += sum;
-#pragma unroll
-        for (int rb = 0; rb < 2; rb++)
-#pragma unroll
-            for (int s2 = 0; s2 < 2; s2++) {
-                bf16x8_t pf;      // a weight is rounded to bfloat16 where it meets the values
-#pragma unroll
-                for (int e = 0; e < 8; e++) pf[e] = (bf16_t)s[rb][8 * s2 + e];
-#pragma unroll
-                for (int db = 0; db < DB; db++) {
-                    const bf16x8_t a = *(const bf16x8_t *)(Vs + (db * 32 + q) * VP + rb * 32 + 16 * s2 + 8 * h);
-                    o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, pf, o[db], 0, 0, 0);
-                }
-            }
-    }
+        }
+        __builtin_amdgcn_s_setprio(0);
+        k0 += KT;
+    };
+    do {
+        while (k0 >= lo_max && k0 <= whole_end && __ballot((unsigned)here >= (unsigned)p.num_pages) == 0) step(std::true_type());      // every row sees all of it
+        if (k0 >= end) break;
+        step(std::false_type());
+    } while (k0 < end);
     __syncthreads();
     if (s_odd && row >= 0) {      // values that are not finite reach the rows that see them here, slot by slot
         for (int slot = begin; slot < end; slot++) {
@@ -277,7 +409,7 @@ tree_wide_kernel(TreeArgs p, TreeSplit sp) {
         const size_t group = ((size_t)seg * nkv + kvh) * sp.tiles + tile;
         const __amdgpu_buffer_rsrc_t meet = workspace_buffer(sp.parts);
         constexpr unsigned kPart = (4 * DB + 1) * THREADS * 16;
-        const unsigned base = (unsigned)(group * sp.splits) * kPart + threadIdx.x * 16, mine = base + split * kPart;
+        const unsigned mine = blockIdx.x * kPart + threadIdx.x * 16;
 #pragma unroll
         for (int db = 0; db < DB; db++)
 #pragma unroll
@@ -298,20 +430,27 @@ tree_wide_kernel(TreeArgs p, TreeSplit sp) {
         for (int db = 0; db < DB; db++)
 #pragma unroll
             for (int i = 0; i < 16; i++) o[db][i] = 0.f;
-        for (int part = 0; part < live; part++) {
-            const unsigned from = base + part * kPart;
-            f32x4_t got[4 * DB];
-            const f32x4_t ml = take_over(meet, from + 4 * DB * THREADS * 16);
+        for (int part = 0; part < live; part += 2) {      // two in one trip
+            f32x4_t got[2][4 * DB], ml[2];
 #pragma unroll
-            for (int i = 0; i < 4 * DB; i++) got[i] = take_over(meet, from + i * THREADS * 16);
-            const float m_new = fmaxf(m, ml[0]);
-            const float f0 = m == -INFINITY ? 0.f : exp2_fast(m - m_new), f1 = ml[0] == -INFINITY ? 0.f : exp2_fast(ml[0] - m_new);
-            m = m_new;
-            l = l * f0 + ml[1] * f1;
+            for (int a = 0; a < 2; a++) {
+                const unsigned from = place.block_of(min(part + a, live - 1) * nkv + kvh) * kPart + threadIdx.x * 16;
+                ml[a] = take_over(meet, from + 4 * DB * THREADS * 16);
 #pragma unroll
-            for (int db = 0; db < DB; db++)
+                for (int i = 0; i < 4 * DB; i++) got[a][i] = take_over(meet, from + i * THREADS * 16);
+            }
 #pragma unroll
-                for (int i = 0; i < 16; i++) o[db][i] = o[db][i] * f0 + got[db * 4 + (i >> 2)][i & 3] * f1;
+            for (int a = 0; a < 2; a++) {
+                if (part + a >= live) break;
+                const float m_new = fmaxf(m, ml[a][0]);
+                const float f0 = m == -INFINITY ? 0.f : exp2_fast(m - m_new), f1 = ml[a][0] == -INFINITY ? 0.f : exp2_fast(ml[a][0] - m_new);
+                m = m_new;
+                l = l * f0 + ml[a][1] * f1;
+#pragma unroll
+                for (int db = 0; db < DB; db++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) o[db][i] = o[db][i] * f0 + got[a][db * 4 + (i >> 2)][i & 3] * f1;
+            }
         }
     }
     if (row < 0) return;
@@ -335,9 +474,9 @@ int launch(const TreeArgs &a, int max_context, hipStream_t stream) {
     TreeSplit sp;
     sp.tiles = (a.max_nodes + TQ - 1) / TQ;
     constexpr size_t part_bytes = (size_t)(4 * (D / 32) + 1) * W * kWave * 16;
-    plan_tree(a, sp.tiles, 8 / W * compute_units(), 64, 8, max_context, part_bytes, &sp);
-    const long units = (long)a.num_segs * sp.splits * a.kv_heads, blocks = (units + 7) / 8 * 8 * sp.tiles;
-    FLLM_REQUIRE(blocks <= 0x7fffffffL, "tree_attention: grid too large");
+    const long places = plan_places(a, 8 / W * compute_units(), 8, part_bytes, &sp);
+    FLLM_REQUIRE(places <= 0x7fffffffL / 8, "tree_attention: grid too large");
+    const long blocks = places * 8;
     hipLaunchKernelGGL((tree_wide_kernel<D, PSH, W>), dim3((unsigned)blocks), dim3(W * kWave), 0, stream, a, sp);
     return fllm_check_launch("tree_attention");
 }

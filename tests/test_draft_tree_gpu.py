@@ -481,3 +481,43 @@ def test_scores_of_minus_infinity(ops, dim, rows, scale, dtype):
         check(ops, case, scale=scale)
     finally:
         ops.set_option("attention.tree_rows", 0)
+
+
+UNEVEN = [(3000, 6), (0, 1), (700, 35), (64, 0), (9, 33), (1500, 17)]
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(4, 1), (16, 2), (6, 3), (8, 4), (16, 8), (9, 9), (60, 20)])
+@pytest.mark.parametrize("window", [0, 1000])
+def test_uneven_requests_share_the_device(ops, heads, kv_heads, window):
+    """The tiles of 128 rows cut the requests by their lengths: any number of key/value heads on the dies, requests without nodes, the same bits
+    each time."""
+    ops.set_option("attention.tree_rows", 128)
+    try:
+        case = plain.TreeCase(UNEVEN, heads, kv_heads, 128, 16, torch.bfloat16, seed=kv_heads)
+        first = check(ops, case, window=window)
+        for _ in range(3):
+            again = attend(ops, case, 128 ** -0.5, window=window).cpu()
+            assert bool((again == first).all())
+        # bounds that the requests do not reach, and a bound on the nodes that cuts some of them
+        check(ops, case, window=window, max_context=100000, max_nodes=64)
+        short = attend(ops, case, 128 ** -0.5, window=window, max_nodes=7).cpu()
+    finally:
+        ops.set_option("attention.tree_rows", 0)
+    for s, (kept, nodes) in enumerate(UNEVEN):
+        row0 = int(case.seg_start[s])
+        assert bool((short[row0 + 7: row0 + nodes] == 7.0).all())
+        want, bound = case.expected(128 ** -0.5, window)
+        assert plain.compare(short[row0: row0 + min(nodes, 7)], want[row0: row0 + min(nodes, 7)], bound[row0: row0 + min(nodes, 7)]) <= 1.0
+
+
+@pytest.mark.parametrize("dim,rows", [(128, 128), (128, 64), (64, 64)])
+def test_many_requests(ops, dim, rows):
+    """More requests and key/value heads than workgroups at a time, one request much longer than the others."""
+    ops.set_option("attention.tree_rows", rows)
+    try:
+        for requests in ([(5 * i % 90, 1 + i % 7) for i in range(70)], [(3 * i % 50, 1 + i % 9) for i in range(39)] + [(4500, 3)] + [(20, 0), (50, 2)]):
+            case = plain.TreeCase(requests, 16, 8, dim, 16, torch.bfloat16, seed=len(requests))
+            first = check(ops, case)
+            assert bool((attend(ops, case, dim ** -0.5).cpu() == first).all())
+    finally:
+        ops.set_option("attention.tree_rows", 0)
