@@ -248,10 +248,8 @@ tree_attention_kernel(TreeArgs p, TreeSplit sp) {
 
     int kb = begin + kw * KB;
     Pages pg = block_pages(kb);
-    if (kb < end) {
 #pragma unroll
-        for (int j = 0; j < KD; j++) load_keys(kb, pg, j);
-    }
+    for (int j = 0; j < KD; j++) load_keys(kb, pg, j);      // behind the end: page 0, for nobody
     if (threadIdx.x == 0) s_odd = 0;
     if ((int)threadIdx.x < ROWS) {
         const int tq = (int)threadIdx.x / G, row = row0 + first_node + tq;
@@ -273,10 +271,9 @@ tree_attention_kernel(TreeArgs p, TreeSplit sp) {
         *(vec *)(qs + r * QP + d) = v;
     }
     __builtin_amdgcn_sched_barrier(0);       // loads come back in order: the scores do not wait for the values
-    if (kb < end) {
+    // (without a condition of their own: where it could have been skipped, keys would be waited for as if no values came after them)
 #pragma unroll
-        for (int dt = 0; dt < DT; dt++) load_values(kb, pg, dt);
-    }
+    for (int dt = 0; dt < DT; dt++) load_values(kb, pg, dt);
     __syncthreads();
     // heads of 64 leave registers for the queries (32 requests of up to 64 nodes at 6,144: 149 -> 144 us); of 128 they stay in LDS
     constexpr bool kHeld = D == 64;
