@@ -28,6 +28,7 @@ struct TreeSplit {
     float *parts;         // [request, key/value head, tile][split][16 NT rows of D outputs, then of a maximum and a sum]
     float scale;          // >= 0: the sign has gone into the queries
     int negate;
+    int sorted;           // requests in the order of their lengths (at most a wave's lanes of them, whole)
 };
 
 __device__ __forceinline__ bf16x8_t pack8(const f32x4_t &lo, const f32x4_t &hi) {
