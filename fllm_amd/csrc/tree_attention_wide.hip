@@ -263,12 +263,14 @@ tree_wide_kernel(TreeArgs p, TreeSplit sp) {
         __syncthreads();   // the previous tile has been read
         if constexpr (!WHOLE) {
             // Slots that no row sees may hold anything, and weights of zero do not keep a NaN or an infinity out: they are cleared, and so is
-            // what is not finite; the rows that see it are given it at the end.
+            // what is not finite; the rows that see it are given it at the end.  A kept slot is at the position of its number; a node is not, and
+            // the window's edge clears none of them.
+            const int low = min(lo_min, kept);
             unsigned odd = 0;
 #pragma unroll
             for (int c = 0; c < CH; c++) {
                 u32x4_t v = __builtin_bit_cast(u32x4_t, vreg[c]);
-                const int from = lo_min <= k0 + v_slot[c] ? 0 : lo_min - (k0 + v_slot[c]), to = (bad >> page_of[c] & 1) ? 0 : n - (k0 + v_slot[c]);
+                const int from = low <= k0 + v_slot[c] ? 0 : low - (k0 + v_slot[c]), to = (bad >> page_of[c] & 1) ? 0 : n - (k0 + v_slot[c]);
 #pragma unroll
                 for (int w = 0; w < 4; w++) {
                     v[w] &= (2 * w >= from && 2 * w < to ? 0x0000ffffu : 0u) | (2 * w + 1 >= from && 2 * w + 1 < to ? 0xffff0000u : 0u);
