@@ -330,6 +330,7 @@ class ModelRunner:
         for g, n in enumerate(need):
             if n > self.cache.free_pages(g):
                 raise OutOfPages(f"the step needs {n} pages of cache group {g}, {self.cache.free_pages(g)} are free")
+        self._tree = None                          # the nodes of this step go where those of the trees before it lie
         for e in entries:
             self.cache.reserve(e.req_id, self.cache.length(e.req_id) + len(e.tokens))
         total = sum(len(e.tokens) for e in entries)

@@ -1,0 +1,92 @@
+"""Steps on trees of drafted tokens and forks on the CPU, with plain kernels: what a request holds after a tree that was left behind, a step that
+failed part of the way, a request that ended meanwhile."""
+import random
+
+import numpy as np
+import pytest
+import torch
+
+import draft_reference as plain
+import plain_llama
+import tiny_configs as tc
+from draft_ops import PlainTreeOps
+from fllm_amd.engine import ModelRunner, StepEntry, StepError, TreeEntry
+from fllm_amd.registry import model_spec_from_config
+from fllm_amd.weights import random_tensors
+
+
+def runner_of(name, max_tokens=400, ops=None, **more):
+    cfg = tc.CONFIGS[name]
+    _, spec = model_spec_from_config(cfg)
+    tensors = random_tensors(spec, 7, torch.float32, with_optional=(name == "C"))
+    args = dict(dtype="float32", device="cpu", page_size=tc.PAGE_SIZES[name], max_tokens=max_tokens, max_requests=8)
+    return ModelRunner(spec, tensors, ops=ops or PlainTreeOps(), **dict(args, **more)), cfg, tc.to_float64(tensors)
+
+
+def free_pages(runner):
+    return [runner.cache.free_pages(g) for g in range(len(runner.cache.groups))]
+
+
+def tree_of(req_id, nodes, vocab, seed=1):
+    rng = random.Random(seed)
+    return TreeEntry(req_id, [rng.randrange(vocab) for _ in range(nodes)], plain.random_tree(nodes, rng))
+
+
+def own_tokens(cfg, weights, tokens, count):
+    """Greedy continuations of `tokens`."""
+    out = []
+    for _ in range(count):
+        out.append(int(np.argmax(plain_llama.forward(cfg, weights, tokens + out)[-1])))
+    return out
+
+
+def next_logits(cfg, weights, tokens, got):
+    want = plain_llama.forward(cfg, weights, tokens)[-1]
+    assert np.abs(got.numpy() - want).max() <= 2e-5 * np.abs(want).max()
+
+
+@pytest.mark.parametrize("name", ["A", "E"])
+def test_a_tree_and_what_is_kept_of_it(name):
+    """Logits of every node, and the next step on what was kept, against the plain implementation."""
+    runner, cfg, weights = runner_of(name)
+    prompt = tc.random_ids(45, cfg["vocab_size"], 1)
+    newest, *more = own_tokens(cfg, weights, prompt, 4)
+    runner.step([StepEntry("a", prompt)])
+    entry = TreeEntry("a", [newest, 3, more[0], 5, more[1], 7], [-1, 0, 0, 2, 2, 4])
+    logits = runner.step_tree([entry])
+    for node, line in enumerate(([], [1], [2], [2, 3], [2, 4], [2, 4, 5])):
+        next_logits(cfg, weights, prompt + [newest] + [entry.tokens[i] for i in line], logits[node])
+    (path, token), = runner.keep_tree(logits.argmax(dim=1).int())
+    assert (path, token) == ([0, 2, 4], more[2]) and runner.length("a") == 48
+    next_logits(cfg, weights, prompt + [newest] + more, runner.step([StepEntry("a", [token], want=(0,))])[0])
+    runner.cache.check_invariants()
+
+
+def failing(runner, monkeypatch, when):
+    """The next forward passes of the model fail, ahead of or behind their launches."""
+    real = runner.model.forward
+
+    def forward(ctx):
+        if when == "after":
+            real(ctx)
+        raise MemoryError("no room for the logits")
+    monkeypatch.setattr(runner.model, "forward", forward)
+
+
+@pytest.mark.parametrize("when", ["before", "after"])
+def test_a_tree_step_that_fails_leaves_the_trees_before_it_behind(monkeypatch, when):
+    """Its nodes may lie in the slots of theirs."""
+    runner, cfg, weights = runner_of("A")
+    prompt = tc.random_ids(21, cfg["vocab_size"], 2)
+    runner.step([StepEntry("a", prompt)])
+    entry = tree_of("a", 6, cfg["vocab_size"])
+    chosen = runner.step_tree([entry]).argmax(dim=1).int()
+    with monkeypatch.context() as patch:
+        failing(runner, patch, when)
+        with pytest.raises(MemoryError):
+            runner.step_tree([tree_of("a", 9, cfg["vocab_size"], seed=5)])
+    with pytest.raises(StepError, match="follows a step_tree"):
+        runner.keep_tree(chosen)
+    assert runner.length("a") == 21
+    runner.cache.check_invariants()
+    next_logits(cfg, weights, prompt + [9], runner.step([StepEntry("a", [9], want=(0,))])[0])
