@@ -376,10 +376,10 @@ class ModelRunner:
         path = torch.empty((S, most), dtype=torch.int32, device=self.device)
         ends = torch.empty((2, S), dtype=torch.int32, device=self.device)
         ops.follow_tree(ctx.ids, ctx.tree.parents, ctx.seg_start, chosen.contiguous(), path, ends[0], ends[1])
+        self._tree = None                         # a path is moved once: where that fails part of the way, nothing is committed
         for g, table in enumerate(ctx.tables):
             v_store = self.model.v_store[g]
             ops.move_tokens(self.model.k_store[g], v_store if v_store.numel() > 0 else None, table, ctx.tree.kept, path, ends[0])
-        self._tree = None
         walked, (lengths, newest) = path.tolist(), ends.tolist()
         out: List[Optional[tuple]] = [None] * S
         for s, i in enumerate(order):

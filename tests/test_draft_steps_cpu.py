@@ -90,3 +90,43 @@ def test_a_tree_step_that_fails_leaves_the_trees_before_it_behind(monkeypatch, w
     assert runner.length("a") == 21
     runner.cache.check_invariants()
     next_logits(cfg, weights, prompt + [9], runner.step([StepEntry("a", [9], want=(0,))])[0])
+
+
+def test_keeping_that_fails_part_of_the_way_is_not_done_twice():
+    """A path that has been moved in one group's pages and is moved again takes other nodes' keys and values."""
+    class Ops(PlainTreeOps):
+        calls, fail_at, refuse = 0, None, False
+
+        def follow_tree(self, *args):
+            if self.refuse:
+                raise ValueError("refused")
+            super().follow_tree(*args)
+
+        def move_tokens(self, *args):
+            self.calls += 1
+            if self.calls == self.fail_at:
+                raise MemoryError("a launch that failed")
+            super().move_tokens(*args)
+
+    ops = Ops()
+    runner, cfg, weights = runner_of("E", ops=ops)
+    assert len(runner.cache.groups) == 2
+    prompt = tc.random_ids(30, cfg["vocab_size"], 3)
+    newest, *more = own_tokens(cfg, weights, prompt, 4)
+    entry = TreeEntry("a", [newest, 3, more[0], 5, more[1]], [-1, 0, 0, 2, 2])
+    runner.step([StepEntry("a", prompt)])
+    chosen = runner.step_tree([entry]).argmax(dim=1).int()
+    ops.refuse = True
+    with pytest.raises(ValueError):
+        runner.keep_tree(chosen)                  # refused ahead of the first move: the trees are still there
+    ops.refuse, ops.fail_at = False, 2
+    with pytest.raises(MemoryError):
+        runner.keep_tree(chosen)
+    with pytest.raises(StepError, match="follows a step_tree"):
+        runner.keep_tree(chosen)
+    assert runner.length("a") == 30 and ops.calls == 2
+    chosen = runner.step_tree([entry]).argmax(dim=1).int()
+    (path, token), = runner.keep_tree(chosen)
+    assert (path, token) == ([0, 2, 4], more[2])
+    next_logits(cfg, weights, prompt + [newest] + more, runner.step([StepEntry("a", [token], want=(0,))])[0])
+    runner.cache.check_invariants()
