@@ -193,22 +193,21 @@ class ModelRunner:
 
     def fork_request(self, src_id, dst_id) -> None:
         """`dst_id` (which must not hold a cache) goes on from what `src_id` has committed: full pages are held by both, a page that is
-        partly filled and the state of fixed size are copied.  Raises `OutOfPages` and changes nothing where the room is not there."""
+        partly filled and the state of fixed size are copied.  Raises `OutOfPages` and changes nothing where the room is not there; where a
+        copy fails `dst_id` holds nothing either."""
         self.cache.length(src_id)                  # an unknown request is refused before anything is added
         self.cache.add_request(dst_id)
         try:
-            copies = self.cache.fork_request(src_id, dst_id)
-        except Exception:
+            for g, copy in enumerate(self.cache.fork_request(src_id, dst_id)):
+                if copy is not None:
+                    stores = [t for t in (self.model.k_store[g], self.model.v_store[g], *(self.model.pool_store[g] or ())) if t.numel() > 0]
+                    self.rt.ops.copy_pages(stores, [copy[0]], [copy[1]])
+            src, dst = self.cache.slot(src_id), self.cache.slot(dst_id)
+            for _, _, arena in self.model.state_arenas():
+                arena[dst].copy_(arena[src])
+        except BaseException:                      # a request whose last page or state was not copied is none
             self.cache.free_request(dst_id)
             raise
-        for g, copy in enumerate(copies):
-            if copy is None:
-                continue
-            stores = [t for t in (self.model.k_store[g], self.model.v_store[g], *(self.model.pool_store[g] or ())) if t.numel() > 0]
-            self.rt.ops.copy_pages(stores, [copy[0]], [copy[1]])
-        src, dst = self.cache.slot(src_id), self.cache.slot(dst_id)
-        for _, _, arena in self.model.state_arenas():
-            arena[dst].copy_(arena[src])
 
     # ---- the step -------------------------------------------------------------------------
     def _validate(self, entries: Sequence[StepEntry], previous_tokens: Optional[torch.Tensor] = None) -> None:

@@ -130,3 +130,40 @@ def test_keeping_that_fails_part_of_the_way_is_not_done_twice():
     assert (path, token) == ([0, 2, 4], more[2])
     next_logits(cfg, weights, prompt + [newest] + more, runner.step([StepEntry("a", [token], want=(0,))])[0])
     runner.cache.check_invariants()
+
+
+@pytest.mark.parametrize("what", ["pages", "state"])
+def test_a_fork_whose_copies_fail_leaves_nothing(monkeypatch, what):
+    """The request that was to go on holds a last page that nobody filled."""
+    class Ops(PlainTreeOps):
+        fails = False
+
+        def copy_pages(self, *args):
+            if self.fails:
+                raise MemoryError("a launch that failed")
+            super().copy_pages(*args)
+
+    ops = Ops()
+    runner, cfg, weights = runner_of("E", ops=ops)
+    prompt = tc.random_ids(37, cfg["vocab_size"], 4)
+    runner.step([StepEntry("a", prompt)])
+    before = free_pages(runner), runner.cache.free_slots()
+
+    def arenas():
+        raise MemoryError("a copy that failed")
+    ops.fails = what == "pages"
+    with monkeypatch.context() as patch:
+        if what == "state":
+            patch.setattr(runner.model, "state_arenas", arenas)
+        with pytest.raises(MemoryError):
+            runner.fork_request("a", "b")
+    assert runner.cache.requests() == ["a"] and (free_pages(runner), runner.cache.free_slots()) == before
+    ops.fails = False
+    with pytest.raises(ValueError):
+        runner.fork_request("a", "a")
+    assert runner.cache.requests() == ["a"]       # a name that is taken is not given up
+    runner.fork_request("a", "b")
+    got = runner.step([StepEntry("a", [3], want=(0,)), StepEntry("b", [8], want=(0,))])
+    next_logits(cfg, weights, prompt + [3], got[0])
+    next_logits(cfg, weights, prompt + [8], got[1])
+    runner.cache.check_invariants()
