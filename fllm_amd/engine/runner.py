@@ -185,7 +185,7 @@ class ModelRunner:
 
     def free_request(self, req_id) -> None:
         if self._tree is not None and any(e.req_id == req_id for e in self._tree[0]):
-            self._tree = None
+            self._leave_trees()
         self.cache.free_request(req_id)
 
     def length(self, req_id) -> int:
@@ -260,10 +260,10 @@ class ModelRunner:
         """Runs the entries as one batch and returns float32 logits [wanted, vocab] on the device,
         in the order of the entries and of each entry's `want`; they are valid until the next step (decode steps
         replay graphs that write them in place).  Unknown requests are added.
-        Raises `OutOfPages` (nothing changed) when the pages do not suffice.
+        Raises `OutOfPages` (nothing changed but that trees of a `step_tree` before it are left behind) when the pages do not suffice.
         `previous_tokens`: the int32 device tensor that entries with `carry` take their token from."""
         self._validate(entries, previous_tokens)
-        self._tree = None
+        self._leave_trees()
         added = []
         try:
             for e in entries:
@@ -302,11 +302,18 @@ class ModelRunner:
         return logits
 
     # ---- trees of drafted tokens ------------------------------------------------------------
+    def _leave_trees(self) -> None:
+        """Leaves the last step's trees behind, if there are any: the pages that hold nothing but their nodes go back."""
+        trees, self._tree = self._tree, None
+        for e in trees[0] if trees is not None else ():
+            if self.cache.has_request(e.req_id):
+                self.cache.trim(e.req_id, self.cache.length(e.req_id))
+
     def step_tree(self, entries: Sequence[TreeEntry]) -> torch.Tensor:
         """Runs trees of drafted tokens as one batch and returns float32 logits [nodes, vocab], entry by entry and node by node: each node's
         in the context of the request's committed tokens and the nodes from the root to it.  Nothing is committed: `keep_tree` keeps the
-        nodes that the model chose itself; any other step leaves the trees behind.  For models whose layers all attend over pages
-        without a chunk, normed heads or biased scores, and keep no state."""
+        nodes that the model chose itself; any other step leaves the trees behind, also one that then finds too few pages (`OutOfPages`)
+        or fails.  For models whose layers all attend over pages without a chunk, normed heads or biased scores, and keep no state."""
         if not all(getattr(self.model.blocks[e.layer].mixer, "takes_trees", False) for e in self.spec.run_order) or self.model.has_state:
             raise StepError("a layer of this model cannot attend over trees of drafted tokens")
         from ..kernels import tree_rows
@@ -322,6 +329,7 @@ class ModelRunner:
         for e in entries:
             if not self.cache.has_request(e.req_id):
                 raise StepError(f"request {e.req_id!r} holds no cache: its prompt is not a tree")
+        self._leave_trees()                        # the nodes of this step go where those of the trees before it lie
         need = [0] * len(self.cache.groups)
         for e in entries:
             for g, m in enumerate(self.cache.pages_missing(e.req_id, self.cache.length(e.req_id) + len(e.tokens))):
@@ -329,9 +337,20 @@ class ModelRunner:
         for g, n in enumerate(need):
             if n > self.cache.free_pages(g):
                 raise OutOfPages(f"the step needs {n} pages of cache group {g}, {self.cache.free_pages(g)} are free")
-        self._tree = None                          # the nodes of this step go where those of the trees before it lie
         for e in entries:
             self.cache.reserve(e.req_id, self.cache.length(e.req_id) + len(e.tokens))
+        try:
+            logits = self._forward_trees(entries, rows)
+        except BaseException:
+            for e in entries:
+                self.cache.trim(e.req_id, self.cache.length(e.req_id))
+            raise
+        self.steps += 1
+        self.rows_total += sum(len(e.tokens) for e in entries)
+        return logits
+
+    def _forward_trees(self, entries: Sequence[TreeEntry], rows: Sequence[tuple]) -> torch.Tensor:
+        """The step itself, behind all checks, and its record for `keep_tree`; `rows`: what `tree_rows` says of every entry."""
         total = sum(len(e.tokens) for e in entries)
         ctx = self._build_context([StepEntry(e.req_id, e.tokens, range(len(e.tokens))) for e in entries])
         # segments of one row lie behind the others: the trees follow the segments
@@ -351,8 +370,6 @@ class ModelRunner:
                             parents=packed[2 * total:3 * total], max_nodes=max(len(e.tokens) for e in entries))
         logits = self.model.forward(ctx)
         self._tree = (list(entries), order, ctx, 1 + max(max(depths) for depths, _ in rows))
-        self.steps += 1
-        self.rows_total += total
         return logits
 
     def keep_tree(self, chosen: torch.Tensor) -> List[tuple]:
@@ -375,11 +392,15 @@ class ModelRunner:
         path = torch.empty((S, most), dtype=torch.int32, device=self.device)
         ends = torch.empty((2, S), dtype=torch.int32, device=self.device)
         ops.follow_tree(ctx.ids, ctx.tree.parents, ctx.seg_start, chosen.contiguous(), path, ends[0], ends[1])
-        self._tree = None                         # a path is moved once: where that fails part of the way, nothing is committed
-        for g, table in enumerate(ctx.tables):
-            v_store = self.model.v_store[g]
-            ops.move_tokens(self.model.k_store[g], v_store if v_store.numel() > 0 else None, table, ctx.tree.kept, path, ends[0])
-        walked, (lengths, newest) = path.tolist(), ends.tolist()
+        try:
+            for g, table in enumerate(ctx.tables):
+                v_store = self.model.v_store[g]
+                ops.move_tokens(self.model.k_store[g], v_store if v_store.numel() > 0 else None, table, ctx.tree.kept, path, ends[0])
+            walked, (lengths, newest) = path.tolist(), ends.tolist()
+        except BaseException:                     # a path is moved once: where that fails part of the way, nothing is committed
+            self._leave_trees()
+            raise
+        self._tree = None
         out: List[Optional[tuple]] = [None] * S
         for s, i in enumerate(order):
             self.cache.commit(entries[i].req_id, lengths[s])

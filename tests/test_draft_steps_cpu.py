@@ -167,3 +167,62 @@ def test_a_fork_whose_copies_fail_leaves_nothing(monkeypatch, what):
     next_logits(cfg, weights, prompt + [3], got[0])
     next_logits(cfg, weights, prompt + [8], got[1])
     runner.cache.check_invariants()
+
+
+@pytest.mark.parametrize("name", ["A", "E"])
+@pytest.mark.parametrize("how", ["step", "step of another", "step_tree", "step_tree of another", "failing step_tree", "free", "free another", "keep"])
+def test_trees_that_are_left_behind_give_their_pages_back(monkeypatch, name, how):
+    runner, cfg, weights = runner_of(name)
+    vocab = cfg["vocab_size"]
+    prompts = {r: tc.random_ids(n, vocab, n) for r, n in (("a", 17), ("b", 30), ("c", 5))}
+    runner.step([StepEntry(r, p) for r, p in prompts.items()])
+    before = free_pages(runner)
+    chosen = runner.step_tree([tree_of("a", 40, vocab), tree_of("b", 40, vocab)]).argmax(dim=1).int()
+    assert all(now < then for now, then in zip(free_pages(runner), before))
+    if how == "step":
+        runner.step([StepEntry("a", [3])])
+    elif how == "step of another":
+        runner.step([StepEntry("c", [3])])
+    elif how == "step_tree":
+        runner.step_tree([tree_of("a", 2, vocab)])
+    elif how == "step_tree of another":
+        runner.step_tree([tree_of("c", 2, vocab)])
+    elif how == "failing step_tree":
+        with monkeypatch.context() as patch:
+            failing(runner, patch, "after")
+            with pytest.raises(MemoryError):
+                runner.step_tree([tree_of("a", 50, vocab), tree_of("c", 40, vocab)])
+    elif how == "free":
+        runner.free_request("a")
+        runner.step([StepEntry("c", [3])])
+    elif how == "free another":
+        runner.free_request("c")
+        runner.step([StepEntry("b", [3])])
+    else:
+        runner.keep_tree(chosen)
+    runner.cache.check_invariants()
+    size = tc.PAGE_SIZES[name]
+    for r in runner.cache.requests():              # no more pages than the tokens of each need, and those of a tree that is still there
+        more = 2 if how == "step_tree" and r == "a" or how == "step_tree of another" and r == "c" else 0
+        for g in range(len(runner.cache.groups)):
+            assert len(runner.cache.table(r, g)) == -(-(runner.length(r) + more) // size), (r, g)
+    if "free" not in how and how != "keep":
+        tail = {"a": [3] if how == "step" else [], "b": [], "c": [3] if how == "step of another" else []}
+        got = runner.step([StepEntry(r, [8], want=(0,)) for r in prompts])
+        for row, (r, p) in zip(got, prompts.items()):
+            next_logits(cfg, weights, p + tail[r] + [8], row)
+
+
+def test_a_step_gets_the_pages_of_trees_that_it_leaves_behind():
+    from fllm_amd.cache import OutOfPages
+    runner, cfg, _ = runner_of("A", max_tokens=6 * 16)
+    vocab = cfg["vocab_size"]
+    runner.step([StepEntry("a", tc.random_ids(10, vocab, 1)), StepEntry("b", tc.random_ids(10, vocab, 2))])
+    runner.step_tree([tree_of("a", 70, vocab)])   # 5 pages of 6, and "b" has the sixth
+    runner.step([StepEntry("b", tc.random_ids(40, vocab, 3))])
+    runner.step_tree([tree_of("a", 20, vocab)])
+    runner.step_tree([tree_of("b", 30, vocab)])   # 80 tokens: five pages, one of them what "a" had for its tree
+    with pytest.raises(OutOfPages):
+        runner.step_tree([tree_of("a", 40, vocab)])
+    assert free_pages(runner) == [1]
+    runner.cache.check_invariants()
