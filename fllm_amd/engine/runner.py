@@ -69,6 +69,16 @@ class TreeEntry:
     parents: Sequence[int]
 
 
+@dataclass
+class _Trees:
+    """What a `step_tree` leaves for `keep_tree`."""
+    entries: List[TreeEntry]
+    order: List[int]               # segment -> entry
+    ctx: StepContext
+    most: int                      # nodes of the longest way from a root
+    held: List[int]                # per entry: tokens that the request's pages could hold ahead of the step
+
+
 class ModelRunner:
     def __init__(self, spec: ModelSpec, tensors: Dict[str, torch.Tensor], dtype="bfloat16", device="cuda:0",
                  page_size: int = 16, max_tokens: Optional[int] = None,
@@ -119,7 +129,7 @@ class ModelRunner:
                                                               max_step_tokens=self.max_step_tokens)
         self.steps = 0
         self.rows_total = 0
-        self._tree: Optional[tuple] = None         # the last step's trees, until `keep_tree` or another step
+        self._tree: Optional[_Trees] = None        # the last step's trees, until `keep_tree` or another step
         # decode steps replay captured graphs when every part can be captured (parts say so with
         # `graph_safe`; a part that decides on the host per step cannot)
         parts_ok = all(getattr(b.mixer, "graph_safe", False)
@@ -184,7 +194,7 @@ class ModelRunner:
         return self.cache.add_request(req_id)
 
     def free_request(self, req_id) -> None:
-        if self._tree is not None and any(e.req_id == req_id for e in self._tree[0]):
+        if self._tree is not None and any(e.req_id == req_id for e in self._tree.entries):
             self._leave_trees()
         self.cache.free_request(req_id)
 
@@ -303,11 +313,16 @@ class ModelRunner:
 
     # ---- trees of drafted tokens ------------------------------------------------------------
     def _leave_trees(self) -> None:
-        """Leaves the last step's trees behind, if there are any: the pages that hold nothing but their nodes go back."""
+        """Leaves the last step's trees behind, if there are any."""
         trees, self._tree = self._tree, None
-        for e in trees[0] if trees is not None else ():
+        if trees is not None:
+            self._trim_trees(trees.entries, trees.held)
+
+    def _trim_trees(self, entries: Sequence[TreeEntry], held: Sequence[int]) -> None:
+        """Gives the pages back that hold nothing but nodes; what was reserved for a request ahead of its tree stays."""
+        for e, tokens in zip(entries, held):
             if self.cache.has_request(e.req_id):
-                self.cache.trim(e.req_id, self.cache.length(e.req_id))
+                self.cache.trim(e.req_id, max(self.cache.length(e.req_id), tokens))
 
     def step_tree(self, entries: Sequence[TreeEntry]) -> torch.Tensor:
         """Runs trees of drafted tokens as one batch and returns float32 logits [nodes, vocab], entry by entry and node by node: each node's
@@ -337,19 +352,19 @@ class ModelRunner:
         for g, n in enumerate(need):
             if n > self.cache.free_pages(g):
                 raise OutOfPages(f"the step needs {n} pages of cache group {g}, {self.cache.free_pages(g)} are free")
+        held = [max((len(self.cache.table(e.req_id, g)) * group.page_size for g, group in enumerate(self.cache.groups)), default=0) for e in entries]
         for e in entries:
             self.cache.reserve(e.req_id, self.cache.length(e.req_id) + len(e.tokens))
         try:
-            logits = self._forward_trees(entries, rows)
+            logits = self._forward_trees(entries, rows, held)
         except BaseException:
-            for e in entries:
-                self.cache.trim(e.req_id, self.cache.length(e.req_id))
+            self._trim_trees(entries, held)
             raise
         self.steps += 1
         self.rows_total += sum(len(e.tokens) for e in entries)
         return logits
 
-    def _forward_trees(self, entries: Sequence[TreeEntry], rows: Sequence[tuple]) -> torch.Tensor:
+    def _forward_trees(self, entries: Sequence[TreeEntry], rows: Sequence[tuple], held: List[int]) -> torch.Tensor:
         """The step itself, behind all checks, and its record for `keep_tree`; `rows`: what `tree_rows` says of every entry."""
         total = sum(len(e.tokens) for e in entries)
         ctx = self._build_context([StepEntry(e.req_id, e.tokens, range(len(e.tokens))) for e in entries])
@@ -369,17 +384,18 @@ class ModelRunner:
         ctx.tree = TreeRows(row_slot=packed[:total], kept=packed[3 * total:], seen=torch.tensor(seen, dtype=torch.int64, device=self.device),
                             parents=packed[2 * total:3 * total], max_nodes=max(len(e.tokens) for e in entries))
         logits = self.model.forward(ctx)
-        self._tree = (list(entries), order, ctx, 1 + max(max(depths) for depths, _ in rows))
+        self._tree = _Trees(list(entries), order, ctx, 1 + max(max(depths) for depths, _ in rows), held)
         return logits
 
     def keep_tree(self, chosen: torch.Tensor) -> List[tuple]:
         """After `step_tree`: `chosen` (int32 [nodes], on the device, in the order of the logits) is the token that the model chose behind every
         node.  Follows the choices from each root to the last node that was drafted, moves the walked nodes' keys and values up behind
-        the committed tokens, commits them and gives back the other nodes' pages.  Returns for every entry (the walked nodes, the
-        request's newest token: what was chosen at the last of them)."""
+        the committed tokens, commits them and gives back the other nodes' pages (not what was reserved ahead of the tree).  Returns for
+        every entry (the walked nodes, the request's newest token: what was chosen at the last of them)."""
         if self._tree is None:
             raise StepError("keep_tree follows a step_tree")
-        entries, order, ctx, most = self._tree
+        trees = self._tree
+        entries, order, ctx, most = trees.entries, trees.order, trees.ctx, trees.most
         rows = sum(len(e.tokens) for e in entries)
         if chosen.shape != (rows,):
             raise StepError(f"{rows} nodes were computed, {tuple(chosen.shape)} tokens are given")
@@ -400,12 +416,11 @@ class ModelRunner:
         except BaseException:                     # a path is moved once: where that fails part of the way, nothing is committed
             self._leave_trees()
             raise
-        self._tree = None
         out: List[Optional[tuple]] = [None] * S
         for s, i in enumerate(order):
             self.cache.commit(entries[i].req_id, lengths[s])
-            self.cache.trim(entries[i].req_id, self.cache.length(entries[i].req_id))
             out[i] = (walked[s][: lengths[s]], newest[s])
+        self._leave_trees()
         return out
 
     # ---- decode steps as HIP graphs ---------------------------------------------------------

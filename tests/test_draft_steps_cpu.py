@@ -226,3 +226,19 @@ def test_a_step_gets_the_pages_of_trees_that_it_leaves_behind():
         runner.step_tree([tree_of("a", 40, vocab)])
     assert free_pages(runner) == [1]
     runner.cache.check_invariants()
+
+
+@pytest.mark.parametrize("end", ["step", "keep"])
+def test_what_was_reserved_ahead_of_a_tree_stays(end):
+    """Pages that the caller has reserved for a request are not a tree's."""
+    runner, cfg, _ = runner_of("A")
+    runner.step([StepEntry("a", tc.random_ids(10, cfg["vocab_size"], 1))])
+    runner.cache.reserve("a", 90)
+    chosen = runner.step_tree([tree_of("a", 100, cfg["vocab_size"])]).argmax(dim=1).int()
+    assert len(runner.cache.table("a", 0)) == 7
+    if end == "step":
+        runner.step([StepEntry("a", [3])])
+    else:
+        runner.keep_tree(chosen)
+    assert len(runner.cache.table("a", 0)) == 6
+    runner.cache.check_invariants()
