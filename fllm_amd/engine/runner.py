@@ -10,7 +10,7 @@ a batch: rust/engine/src/runtime.rs:2380-2442).
 from __future__ import annotations
 
 import gc
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 from typing import Dict, List, Optional, Sequence, Union
 
 import torch
@@ -77,6 +77,7 @@ class _Trees:
     ctx: StepContext
     most: int                      # nodes of the longest way from a root
     held: List[int]                # per entry: tokens that the request's pages could hold ahead of the step
+    ended: set = field(default_factory=set)      # entries whose requests have ended since
 
 
 class ModelRunner:
@@ -194,8 +195,8 @@ class ModelRunner:
         return self.cache.add_request(req_id)
 
     def free_request(self, req_id) -> None:
-        if self._tree is not None and any(e.req_id == req_id for e in self._tree.entries):
-            self._leave_trees()
+        if self._tree is not None:                 # the other requests' trees are still there
+            self._tree.ended.update(i for i, e in enumerate(self._tree.entries) if e.req_id == req_id)
         self.cache.free_request(req_id)
 
     def length(self, req_id) -> int:
@@ -316,7 +317,8 @@ class ModelRunner:
         """Leaves the last step's trees behind, if there are any."""
         trees, self._tree = self._tree, None
         if trees is not None:
-            self._trim_trees(trees.entries, trees.held)
+            live = [i for i in range(len(trees.entries)) if i not in trees.ended]
+            self._trim_trees([trees.entries[i] for i in live], [trees.held[i] for i in live])
 
     def _trim_trees(self, entries: Sequence[TreeEntry], held: Sequence[int]) -> None:
         """Gives the pages back that hold nothing but nodes; what was reserved for a request ahead of its tree stays."""
@@ -391,7 +393,8 @@ class ModelRunner:
         """After `step_tree`: `chosen` (int32 [nodes], on the device, in the order of the logits) is the token that the model chose behind every
         node.  Follows the choices from each root to the last node that was drafted, moves the walked nodes' keys and values up behind
         the committed tokens, commits them and gives back the other nodes' pages (not what was reserved ahead of the tree).  Returns for
-        every entry (the walked nodes, the request's newest token: what was chosen at the last of them)."""
+        every entry (the walked nodes, the request's newest token: what was chosen at the last of them); ([], -1) for a request that
+        `free_request` has ended meanwhile."""
         if self._tree is None:
             raise StepError("keep_tree follows a step_tree")
         trees = self._tree
@@ -408,8 +411,11 @@ class ModelRunner:
         path = torch.empty((S, most), dtype=torch.int32, device=self.device)
         ends = torch.empty((2, S), dtype=torch.int32, device=self.device)
         ops.follow_tree(ctx.ids, ctx.tree.parents, ctx.seg_start, chosen.contiguous(), path, ends[0], ends[1])
+        ended = [s for s, i in enumerate(order) if i in trees.ended]
         try:
             for g, table in enumerate(ctx.tables):
+                for s in ended:                   # its pages may be another request's by now: none of its slots has one
+                    table[s].fill_(-1)
                 v_store = self.model.v_store[g]
                 ops.move_tokens(self.model.k_store[g], v_store if v_store.numel() > 0 else None, table, ctx.tree.kept, path, ends[0])
             walked, (lengths, newest) = path.tolist(), ends.tolist()
@@ -418,6 +424,9 @@ class ModelRunner:
             raise
         out: List[Optional[tuple]] = [None] * S
         for s, i in enumerate(order):
+            if s in ended:
+                out[i] = ([], -1)
+                continue
             self.cache.commit(entries[i].req_id, lengths[s])
             out[i] = (walked[s][: lengths[s]], newest[s])
         self._leave_trees()

@@ -242,3 +242,39 @@ def test_what_was_reserved_ahead_of_a_tree_stays(end):
         runner.keep_tree(chosen)
     assert len(runner.cache.table("a", 0)) == 6
     runner.cache.check_invariants()
+
+
+@pytest.mark.parametrize("again", [False, True])
+@pytest.mark.parametrize("ended", [["a"], ["b"], ["c"], ["a", "c"], ["a", "b", "c"], ["d"]])
+def test_requests_that_end_between_a_tree_and_what_is_kept_of_it(ended, again):
+    """The other requests' nodes are kept; pages that have gone to other requests since are not written."""
+    runner, cfg, weights = runner_of("E", max_tokens=16 * 16)
+    vocab = cfg["vocab_size"]
+    prompts = {r: tc.random_ids(n, vocab, n) for r, n in (("a", 17), ("b", 30), ("c", 5), ("d", 4))}
+    runner.step([StepEntry(r, p) for r, p in prompts.items()])
+    own = {r: own_tokens(cfg, weights, prompts[r], 4) for r in "abc"}
+    entries = [TreeEntry(r, [t[0], 3, t[1], 5, t[2]], [-1, 0, 0, 2, 2]) for r, t in own.items()]
+    entries[1] = TreeEntry("b", own["b"][:1], [-1])           # one node: its segment lies behind the others
+    chosen = runner.step_tree(entries).argmax(dim=1).int()
+    for r in ended:
+        runner.free_request(r)
+        if again:                                             # a new request of the same name, in the pages that are free now
+            runner.add_request(r)
+    pages = [runner.model.k_store[g].clone() for g in range(2)]
+    held = [{p for r in runner.cache.requests() for p in runner.cache.table(r, g) if p >= 0} for g in range(2)]
+    kept = runner.keep_tree(chosen)
+    for g in range(2):
+        for page in set(range(pages[g].shape[1])) - held[g]:
+            assert torch.equal(runner.model.k_store[g][:, page], pages[g][:, page])
+    for entry, got in zip(entries, kept):
+        r = entry.req_id
+        if r in ended:
+            assert got == ([], -1) and (runner.length(r) == 0 if again else not runner.cache.has_request(r))
+            continue
+        nodes = [0] if r == "b" else [0, 2, 4]
+        assert got == (nodes, own[r][len(nodes)]) and runner.length(r) == len(prompts[r]) + len(nodes)
+        row, = runner.step([StepEntry(r, [got[1]], want=(0,))])
+        next_logits(cfg, weights, prompts[r] + own[r][: len(nodes) + 1], row)
+    runner.cache.check_invariants()
+    with pytest.raises(StepError):
+        runner.keep_tree(chosen)
