@@ -482,12 +482,12 @@ class Ops:
         at zero, partial results behind them), so launches on one device must not overlap: all of them go to one stream
         (a stream that is capturing a graph stands for the stream the graph will be replayed on).  A launch on a second
         stream of the same device is refused."""
-        return Ops._stream_and_device()[0]
+        return Ops._launch_on(*Ops._current_stream())
 
     @staticmethod
-    def _stream_and_device() -> Tuple[int, int]:
-        """What `_stream` gives, and the device it is of."""
-        device, handle = Ops._current_stream()
+    def _launch_on(device: int, handle: int) -> int:
+        """The handle, unless the device's kernels belong to another stream (`_stream`).  Asked for behind a call's own checks: the
+        first launch makes its stream the device's."""
         seen = Ops._streams.get(device)
         if seen is None:
             if not torch.cuda.is_current_stream_capturing():
@@ -495,7 +495,7 @@ class Ops:
         elif handle != seen and not torch.cuda.is_current_stream_capturing():
             raise KernelError(f"kernels of device {device} were launched on stream {seen:#x} before and are now asked for on "
                               f"stream {handle:#x}: they share the device workspace and must stay on one stream")
-        return handle, device
+        return handle
 
     @staticmethod
     def _on_the_kernels_stream() -> bool:
@@ -2063,7 +2063,7 @@ class Ops:
         _need(q.dim() == 2 and tables.dim() == 2 and seen.dim() == 2, "q must be [rows, lanes], tables [segments, pages], seen [rows, words]")
         rows, width = q.shape
         v_dim = head_dim if v_dim is None else int(v_dim)
-        stream, device = self._stream_and_device()
+        device, stream = self._current_stream()
         dtype = q.dtype
         if not (q.is_cuda and q.stride(1) == 1 and width == heads * head_dim):
             raise KernelError(f"q must be [rows, {heads * head_dim}] with unit column stride")
@@ -2084,7 +2084,7 @@ class Ops:
             _held(kept, "kept", device, torch.int32, (segs,)), _held(seen, "seen", device, torch.int64, (rows, words)), words,
             _held(out, "out", device, dtype, (rows, heads * v_dim)), rows, heads, kv_heads, head_dim, v_dim, page_size, num_pages,
             float(scale), int(window) if window else 0, key_chunk, None if sinks is None else _held(sinks, "sinks", device, torch.float32, (heads,)),
-            _DTYPE_CODE[dtype], min(most, rows), int(max_context), stream))
+            _DTYPE_CODE[dtype], min(most, rows), int(max_context), self._launch_on(device, stream)))
         return out
 
     def follow_tree(self, drafted: torch.Tensor, parents: torch.Tensor, seg_start: torch.Tensor, chosen: torch.Tensor, path: torch.Tensor,
@@ -2094,7 +2094,7 @@ class Ops:
         the walk goes to the lowest child whose token is what was chosen at its parent.  `path` (int32 [segments, n], n the most nodes
         wanted): its nodes, -1 behind them; `length`: how many; `newest`: what was chosen at the last, the request's next token.  A
         segment without rows: length 0, newest -1."""
-        stream, device = self._stream_and_device()
+        device, stream = self._current_stream()
         _need(drafted.dim() == 1 and path.dim() == 2, "drafted must be [rows], path [segments, nodes]")
         (rows,), (segs, most), i32 = drafted.shape, path.shape, torch.int32
         _need(most > 0, "path must have room for a node")
@@ -2102,7 +2102,7 @@ class Ops:
             _held(drafted, "drafted", device, i32, (rows,)), _held(parents, "parents", device, i32, (rows,)),
             _held(seg_start, "seg_start", device, i32, (segs + 1,)), segs, _held(chosen, "chosen", device, i32, (rows,)), rows,
             _held(path, "path", device, i32, (segs, most)), most, _held(length, "length", device, i32, (segs,)),
-            _held(newest, "newest", device, i32, (segs,)), stream))
+            _held(newest, "newest", device, i32, (segs,)), self._launch_on(device, stream)))
 
     def move_tokens(self, k_store: torch.Tensor, v_store: Optional[torch.Tensor], tables: torch.Tensor, kept: torch.Tensor, path: torch.Tensor,
                     length: torch.Tensor) -> None:
@@ -2111,7 +2111,7 @@ class Ops:
         `k_store` [layers, pages, kv_heads, k_dim / chunk, page_size, chunk] (or [layers, pages, kv_heads, page_size, k_dim]) and
         `v_store` [layers, pages, kv_heads, v_dim, page_size] (None where keys are all there is): the pages of all layers that share the
         block tables `tables` [segments, pages].  Slots without a page are left out."""
-        stream, device = self._stream_and_device()
+        device, stream = self._current_stream()
         shape, dtype, i32 = k_store.shape, k_store.dtype, torch.int32
         _need(len(shape) in (5, 6), "k_store must be [layers, pages, kv_heads, k_dim / chunk, page_size, chunk]")
         if dtype not in _DTYPE_CODE:
@@ -2130,13 +2130,14 @@ class Ops:
             None if v_store is None else _held(v_store, "v_store", device, dtype, (layers, pages, kv_heads, v_dim, page_size)),
             layers, pages, kv_heads, chunk * (shape[3] if len(shape) == 6 else 1), v_dim, page_size, chunk, 4 if dtype is torch.float32 else 2,
             _held(tables, "tables", device, i32, (segs, stride)), stride, segs, _held(kept, "kept", device, i32, (segs,)),
-            _held(path, "path", device, i32, (segs, most)), most, _held(length, "length", device, i32, (segs,)), stream))
+            _held(path, "path", device, i32, (segs, most)), most, _held(length, "length", device, i32, (segs,)),
+            self._launch_on(device, stream)))
 
     def copy_pages(self, stores: Sequence[torch.Tensor], source: Sequence[int], target: Sequence[int]) -> None:
         """Page source[i] is copied to page target[i] in every layer of every store ([layers, pages, ...], at most 8 of them): what a request
         takes over of another's when it goes on from the same tokens (`CacheManager.fork_request` names the pages), or a cache that is
         packed.  No page is a target twice, or a source and a target."""
-        stream, device = self._stream_and_device()
+        device, stream = self._current_stream()
         pairs, count = len(source), len(stores)
         if len(target) != pairs:
             raise KernelError(f"{pairs} pages to copy from, {len(target)} to copy to")
@@ -2160,7 +2161,8 @@ class Ops:
             return
         i64, i32 = ctypes.c_int64 * count, ctypes.c_int32 * pairs
         counts = [i64(*column) for column in zip(*sizes)]
-        self._check(self.lib.fllm_copy_pages((ctypes.c_void_p * count)(*addresses), *counts, count, i32(*source), i32(*target), pairs, stream))
+        self._check(self.lib.fllm_copy_pages((ctypes.c_void_p * count)(*addresses), *counts, count, i32(*source), i32(*target), pairs,
+                                             self._launch_on(device, stream)))
 
     # ---- attention over cached latents ------------------------------------------------------------------------------------
     def latent_rope_store(self, joint: torch.Tensor, dkv_at: int, rank: int, rot: int, c_weight: torch.Tensor, eps: float, heads: int, dim: int,
