@@ -12,6 +12,7 @@ import functools
 import math
 import threading
 import weakref
+from operator import index as _whole
 from typing import Dict, NamedTuple, Optional, Sequence, Tuple
 
 import torch
@@ -2136,8 +2137,9 @@ class Ops:
     def copy_pages(self, stores: Sequence[torch.Tensor], source: Sequence[int], target: Sequence[int]) -> None:
         """Page source[i] is copied to page target[i] in every layer of every store ([layers, pages, ...], at most 8 of them): what a request
         takes over of another's when it goes on from the same tokens (`CacheManager.fork_request` names the pages), or a cache that is
-        packed.  No page is a target twice, or a source and a target."""
+        packed.  No page is a target twice, or a source and a target.  The page numbers are the host's (anything that is a whole number)."""
         device, stream = self._current_stream()
+        source, target = list(map(_whole, source)), list(map(_whole, target))      # numbers: two tensors of one value are not equal to a set
         pairs, count = len(source), len(stores)
         if len(target) != pairs:
             raise KernelError(f"{pairs} pages to copy from, {len(target)} to copy to")

@@ -44,3 +44,34 @@ def test_copying_nothing_does_not_choose_the_stream(ops, monkeypatch):
     monkeypatch.setattr("fllm_amd.kernels._held", lambda t, *_: t.data_ptr())
     ops.copy_pages((torch.zeros((1, 3, 8)),), [], [])
     assert Ops._streams == {}
+
+
+@pytest.mark.parametrize("kind", [list, tuple, torch.tensor, np.array, lambda v: [torch.tensor(p) for p in v]], ids=["list", "tuple", "tensor", "array", "tensors"])
+def test_pages_that_meet_are_refused_in_whatever_they_are_given(ops, kind):
+    """Two pairs that write one page, or one that reads what another writes, run at the same time: which is first is anyone's guess."""
+    store = (torch.zeros((1, 9, 8)),)
+    for source, target, message in (([0, 1], [2, 2], "copied to twice"), ([0, 1], [1, 2], "copied from and to"), ([0, 1], [2, 9], "has 9 pages"), ([0, -1], [2, 3], "has 9 pages")):
+        with pytest.raises(KernelError, match=message if "has" not in message else "must be on the GPU|has 9 pages"):
+            ops.copy_pages(store, kind(source), kind(target))
+
+
+def test_page_numbers_are_whole(ops):
+    for wrong in ([0.0], [0.5], ["0"], [None]):
+        with pytest.raises((KernelError, TypeError)):
+            ops.copy_pages((torch.zeros((1, 9, 8)),), wrong, [1])
+        with pytest.raises((KernelError, TypeError)):
+            ops.copy_pages((torch.zeros((1, 9, 8)),), [1], wrong)
+
+
+@pytest.mark.parametrize("kind", [list, torch.tensor, np.array], ids=["list", "tensor", "array"])
+def test_pages_that_do_not_meet_are_copied(ops, monkeypatch, kind):
+    seen = []
+
+    class Library:
+        def fllm_copy_pages(self, stores, layers, pages, sizes, count, source, target, pairs, stream):
+            seen.append((list(layers), list(pages), list(sizes), count, list(source), list(target), pairs, stream))
+            return 0
+    ops.lib = Library()
+    monkeypatch.setattr("fllm_amd.kernels._held", lambda t, *_: t.data_ptr())
+    ops.copy_pages((torch.zeros((2, 9, 8)), torch.zeros((3, 10, 4), dtype=torch.bfloat16)), kind([0, 0, 5]), kind([1, 8, 2]))
+    assert seen == [([2, 3], [9, 10], [32, 8], 2, [0, 0, 5], [1, 8, 2], 3, 0x1234)]
