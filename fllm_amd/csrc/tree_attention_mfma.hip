@@ -22,7 +22,7 @@
 #include "draft_api.h"
 #include "tree_attention.h"
 
-int fllm_tree_attention_wide(const TreeArgs &a, int max_context, hipStream_t stream);      // tree_attention_wide.hip
+int fllm_tree_attention_wide(const TreeArgs &a, hipStream_t stream);      // tree_attention_wide.hip
 
 namespace {
 
@@ -71,8 +71,7 @@ __global__ void __launch_bounds__(RG * KW * kWave) __attribute__((amdgpu_waves_p
 tree_attention_kernel(TreeArgs p, TreeSplit sp) {
     typedef typename Operand<T>::vec vec;
     constexpr bool kHalf = sizeof(T) == 2;
-    constexpr int H = 1;                    // value loads of all lanes a block
-    constexpr int PER = Operand<T>::kPer, KB = Operand<T>::kStep * H, TILES = KB / 16, THREADS = RG * KW * kWave;
+    constexpr int PER = Operand<T>::kPer, KB = Operand<T>::kStep, TILES = KB / 16, THREADS = RG * KW * kWave;
     constexpr int KD = D / (4 * PER);       // 16-byte loads of a key a lane
     constexpr bool P8 = PSH == 3;
     constexpr int PS = 1 << PSH, PMASK = PS - 1;
@@ -151,12 +150,12 @@ tree_attention_kernel(TreeArgs p, TreeSplit sp) {
         }
         return pg;
     };
-    vec kf[TILES][KD], vf[H][DT];
+    vec kf[TILES][KD], vf[DT];
     // A lane's place in a page is the same in every block; the rest of an address is a scalar wherever one page serves all lanes.
     constexpr size_t kHeadBytes = (size_t)D * PS * sizeof(T);
     // Rows of the score tiles.  A tile alone reads a key once, from memory: row c of score tile k is slot 16 k + c, a load is whole lines, carries
     // the non-temporal hint, and probabilities change lanes for it.  Where several tiles read the same keys most come from L2, and what
-    // counts is the instructions: row c of score tile k of a step of 32 slots is slot 8 (c / 4) + 4 (k % 2) + c % 4, so that a lane's
+    // counts is the instructions: row c of score tile k is slot 8 (c / 4) + 4 (k % 2) + c % 4, so that a lane's
     // scores are of the neighbouring slots that its values are of.  Microseconds with one order and the hint / with the other: 8 requests
     // of 8 nodes at 16,000 kept tokens 62 / 75; of 26 nodes at 2,000 (4 tiles a key/value head) 23.6 / 19.8.
     constexpr bool kSwap = kHalf && ALONE, kNear = kHalf && !ALONE;
@@ -169,10 +168,9 @@ tree_attention_kernel(TreeArgs p, TreeSplit sp) {
         for (int t = 0; t < TILES; t++) {
             const char *base = (const char *)p.kp + (size_t)kvh * kHeadBytes;
             if constexpr (kNear) {
-                const int h = t >> 1;
-                if constexpr (P8) base += (size_t)(c < 8 ? (c < 4 ? pg.page[4 * h] : pg.page[4 * h + 1]) : (c < 12 ? pg.page[4 * h + 2] : pg.page[4 * h + 3])) * page_bytes;
-                else if constexpr (PSH == 4) base += (size_t)(c < 8 ? pg.page[2 * h] : pg.page[2 * h + 1]) * page_bytes;
-                else base += (size_t)pg.page[2 * h] * page_bytes + (size_t)((kb + 32 * h) & PMASK) * 16;
+                if constexpr (P8) base += (size_t)(c < 8 ? (c < 4 ? pg.page[0] : pg.page[1]) : (c < 12 ? pg.page[2] : pg.page[3])) * page_bytes;
+                else if constexpr (PSH == 4) base += (size_t)(c < 8 ? pg.page[0] : pg.page[1]) * page_bytes;
+                else base += (size_t)pg.page[0] * page_bytes + (size_t)(kb & PMASK) * 16;
                 base += (t & 1) * 64;
             } else {
                 if constexpr (P8) base += (size_t)(c < 8 ? pg.page[2 * t] : pg.page[2 * t + 1]) * page_bytes;
@@ -183,24 +181,16 @@ tree_attention_kernel(TreeArgs p, TreeSplit sp) {
             else kf[t][j] = *from;
         }
     };
-    // values: bfloat16 the slots 32 h + 8 g .. + 7, float32 16 h + 4 g .. + 3
+    // values: bfloat16 the slots 8 g .. + 7 of a block, float32 4 g .. + 3
     const unsigned v_lane = (unsigned)(c * PS + (kHalf ? (P8 ? 0 : PSH == 4 ? 8 * (g & 1) : 8 * g) : (P8 ? 4 * (g & 1) : 4 * g))) * (unsigned)sizeof(T);
     // lanes 16 dt .. 16 dt + 15 of a block's values
     auto load_values = [&](int kb, const Pages &pg, int dt) __attribute__((always_inline)) {
-#pragma unroll
-        for (int h = 0; h < H; h++) {
-            const char *base = (const char *)p.vp + (size_t)kvh * kHeadBytes;
-            const size_t page_bytes = (size_t)nkv * kHeadBytes;
-            if constexpr (kHalf) {
-                if constexpr (P8) base += (size_t)(g < 2 ? (g == 0 ? pg.page[4 * h] : pg.page[4 * h + 1]) : (g == 2 ? pg.page[4 * h + 2] : pg.page[4 * h + 3])) * page_bytes;
-                else if constexpr (PSH == 4) base += (size_t)(g < 2 ? pg.page[2 * h] : pg.page[2 * h + 1]) * page_bytes;
-                else base += (size_t)pg.page[2 * h] * page_bytes + (size_t)((kb + 32 * h) & PMASK) * sizeof(T);
-            } else {
-                if constexpr (P8) base += (size_t)(g < 2 ? pg.page[2 * h] : pg.page[2 * h + 1]) * page_bytes;
-                else base += (size_t)pg.page[h] * page_bytes + (size_t)((kb + 16 * h) & PMASK) * sizeof(T);
-            }
-            vf[h][dt] = *(const vec *)(base + dt * 16 * PS * (int)sizeof(T) + v_lane);
-        }
+        const char *base = (const char *)p.vp + (size_t)kvh * kHeadBytes;
+        const size_t page_bytes = (size_t)nkv * kHeadBytes;
+        if constexpr (kHalf && P8) base += (size_t)(g < 2 ? (g == 0 ? pg.page[0] : pg.page[1]) : (g == 2 ? pg.page[2] : pg.page[3])) * page_bytes;
+        else if constexpr (kHalf ? PSH == 4 : P8) base += (size_t)(g < 2 ? pg.page[0] : pg.page[1]) * page_bytes;
+        else base += (size_t)pg.page[0] * page_bytes + (size_t)(kb & PMASK) * sizeof(T);
+        vf[dt] = *(const vec *)(base + dt * 16 * PS * (int)sizeof(T) + v_lane);
     };
     // The words of a block's nodes for the lane's row of tile t: the one that holds the first (bit j0 % 64) and the one behind it.
     struct Words {
@@ -285,7 +275,7 @@ tree_attention_kernel(TreeArgs p, TreeSplit sp) {
 #pragma unroll
     for (int dt = 0; dt < DT; dt++) load_values(kb, pg, dt);
     __syncthreads();
-    // heads of 64 leave registers for the queries (32 requests of up to 64 nodes at 6,144: 149 -> 144 us); of 128 they stay in LDS
+    // heads of 64 leave registers for the queries (32 requests of up to 64 nodes at 6,144: 134 -> 128 us); of 128 they stay in LDS
     constexpr bool kHeld = D == 64;
     vec qf[kHeld ? NT : 1][KD];
     if constexpr (kHeld) {
@@ -381,7 +371,7 @@ tree_attention_kernel(TreeArgs p, TreeSplit sp) {
                 m_run[t] = m_new;
             }
         }
-        vec pv[NT][H];        // the weights as the second product takes them
+        vec pv[NT];        // the weights as the second product takes them
 #pragma unroll
         for (int t = 0; t < NT; t++) {
             const float mc = m_run[t] * sc;      // finite for a row that has seen nothing
@@ -394,12 +384,10 @@ tree_attention_kernel(TreeArgs p, TreeSplit sp) {
                     sum += s[t][k][i];
                 }
             l_run[t] += sum;
-#pragma unroll
-            for (int h = 0; h < H; h++) {
-                if constexpr (kSwap) pv[t][h] = neighbours(pack8(s[t][2 * h], s[t][2 * h + 1]));
-                else if constexpr (kHalf) pv[t][h] = pack8(s[t][2 * h], s[t][2 * h + 1]);      // rounded to bfloat16 where they meet the values
-                else pv[t][h] = s[t][h];
-            }
+            // rounded to bfloat16 where they meet the values, which the matrix instruction takes in one type; sums stay in float32
+            if constexpr (kSwap) pv[t] = neighbours(pack8(s[t][0], s[t][1]));
+            else if constexpr (kHalf) pv[t] = pack8(s[t][0], s[t][1]);
+            else pv[t] = s[t][0];
         }
         if constexpr (!WHOLE) {
             // Slots that nobody sees may hold anything, and weights of zero do not keep a NaN or an infinity out: they are cleared.
@@ -407,52 +395,45 @@ tree_attention_kernel(TreeArgs p, TreeSplit sp) {
 #pragma unroll
             for (int step = 8; step > 0; step >>= 1) any |= __shfl_xor(any, step);
             unsigned odd = 0;
+            const unsigned mine = (unsigned)(any >> (PER * g));
+            u32x4_t keep;
 #pragma unroll
-            for (int h = 0; h < H; h++) {
-                const unsigned mine = (unsigned)(any >> (4 * PER * h + PER * g));
-                u32x4_t keep;
+            for (int w = 0; w < 4; w++) {
+                if constexpr (kHalf) keep[w] = (mine >> (2 * w) & 1 ? 0x0000ffffu : 0u) | (mine >> (2 * w + 1) & 1 ? 0xffff0000u : 0u);
+                else keep[w] = mine >> w & 1 ? ~0u : 0u;
+            }
 #pragma unroll
-                for (int w = 0; w < 4; w++) {
-                    if constexpr (kHalf) keep[w] = (mine >> (2 * w) & 1 ? 0x0000ffffu : 0u) | (mine >> (2 * w + 1) & 1 ? 0xffff0000u : 0u);
-                    else keep[w] = mine >> w & 1 ? ~0u : 0u;
-                }
+            for (int dt = 0; dt < DT; dt++) {
+                const u32x4_t v = __builtin_bit_cast(u32x4_t, vf[dt]) & keep;
+                vf[dt] = __builtin_bit_cast(vec, v);
 #pragma unroll
-                for (int dt = 0; dt < DT; dt++) {
-                    const u32x4_t v = __builtin_bit_cast(u32x4_t, vf[h][dt]) & keep;
-                    vf[h][dt] = __builtin_bit_cast(vec, v);
-#pragma unroll
-                    for (int w = 0; w < 4; w++) odd |= (v[w] & kExponents) + kExponentStep;       // a full exponent carries into the sign's place
-                }
+                for (int w = 0; w < 4; w++) odd |= (v[w] & kExponents) + kExponentStep;       // a full exponent carries into the sign's place
             }
             if (__any((odd & kSigns) != 0)) {
                 if (lane == 0) s_odd = 1;
 #pragma unroll
-                for (int h = 0; h < H; h++)
+                for (int dt = 0; dt < DT; dt++) {
+                    u32x4_t v = __builtin_bit_cast(u32x4_t, vf[dt]);
 #pragma unroll
-                    for (int dt = 0; dt < DT; dt++) {
-                        u32x4_t v = __builtin_bit_cast(u32x4_t, vf[h][dt]);
-#pragma unroll
-                        for (int w = 0; w < 4; w++) {
-                            const unsigned full = ((v[w] & kExponents) + kExponentStep) & kSigns;      // the sign bits of what is not finite
-                            v[w] &= ~(kHalf ? ((full >> 15) * 0xffffu) : ((full >> 31) * 0xffffffffu));
-                        }
-                        vf[h][dt] = __builtin_bit_cast(vec, v);
+                    for (int w = 0; w < 4; w++) {
+                        const unsigned full = ((v[w] & kExponents) + kExponentStep) & kSigns;      // the sign bits of what is not finite
+                        v[w] &= ~(kHalf ? ((full >> 15) * 0xffffu) : ((full >> 31) * 0xffffffffu));
                     }
+                    vf[dt] = __builtin_bit_cast(vec, v);
+                }
             }
         }
 #pragma unroll
         for (int dt = 0; dt < DT; dt++) {
 #pragma unroll
-            for (int t = 0; t < NT; t++)
+            for (int t = 0; t < NT; t++) {
+                if constexpr (kHalf) {
+                    o[t][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[dt], pv[t], o[t][dt], 0, 0, 0);
+                } else {
 #pragma unroll
-                for (int h = 0; h < H; h++) {
-                    if constexpr (kHalf) {
-                        o[t][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[h][dt], pv[t][h], o[t][dt], 0, 0, 0);
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 4; e++) o[t][dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[h][dt][e], pv[t][h][e], o[t][dt], 0, 0, 0);
-                    }
+                    for (int e = 0; e < 4; e++) o[t][dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[dt][e], pv[t][e], o[t][dt], 0, 0, 0);
                 }
+            }
             load_values(next, pg, dt);
         }
         kb = next;
@@ -660,7 +641,7 @@ int launch_rows(const TreeArgs &a, int max_context, hipStream_t stream) {
         const bool much = tiles32 * (double)reach > (D == 128 ? 1500000 : 900000);
         if (G <= 32 && (asked ? asked <= 32 : rows <= 32 || (tiles32 <= compute_units() && !much))) return go(two(), one(), eight());
         if constexpr (D == 64) return go(four(), one(), eight());
-        else if (asked ? asked == 128 : much || tiles_of(64) >= 2 * compute_units()) return fllm_tree_attention_wide(a, max_context, stream);
+        else if (asked ? asked == 128 : much || tiles_of(64) >= 2 * compute_units()) return fllm_tree_attention_wide(a, stream);
         else return go(two(), two(), four());
     }
 }

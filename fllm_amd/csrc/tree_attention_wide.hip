@@ -1,6 +1,6 @@
 // Attention of large trees of drafted tokens on the matrix cores (bfloat16): many rows share every key.
 //
-// A workgroup of W waves takes 32 W rows (nodes x the query heads of one key/value head) and a stretch of the request's slots; keys and
+// A workgroup of four waves takes 128 rows (nodes x the query heads of one key/value head) and a stretch of the request's slots; keys and
 // values go through LDS in tiles of 64 slots, the next tile on its way into registers while the waves multiply the current one, each 32
 // rows of its own:
 //   S^T[key][row] = K[key][:] . Q[row][:]          O^T[d][row] += V^T[d][key] P^T[key][row]          (v_mfma_f32_32x32x16_bf16)
@@ -137,14 +137,17 @@ long plan_places(const TreeArgs &a, int slots, int least, size_t part_bytes, Tre
     return std::max((long)a.num_segs * ((a.kv_heads + 7) / 8) * sp->tiles, sp->places + rounded);
 }
 
-template <int D, int PSH, int W>
-__global__ void __launch_bounds__(W * kWave) __attribute__((amdgpu_waves_per_eu(2, 2)))
+constexpr int D = 128, W = 4, THREADS = W * kWave, ROWS = 32 * W;       // lanes of a head, waves, rows of a tile
+
+// PSH: pages of 1 << PSH tokens
+template <int PSH>
+__global__ void __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(2, 2)))
 tree_wide_kernel(TreeArgs p, TreeSplit sp) {
-    constexpr int THREADS = W * kWave, ROWS = 32 * W, KT = 64, PS = 1 << PSH, PAGES = KT / PS;
+    constexpr int KT = 64, PS = 1 << PSH, PAGES = KT / PS;
     constexpr int KP = D + 8, VP = KT + 8;           // pitches of a key (D values) and of a lane of the values (KT slots) in LDS
     constexpr int DS = D / 16, DB = D / 32, CH = KT * D / 8 / THREADS;      // 16-byte chunks a thread and tile, keys and values each
-    constexpr int LD = D == 64 ? 6 : 7, LPC = LD + PSH - 3;      // log2 of D and of a page's chunks
-    static_assert(CH >= 1 && LPC >= 6, "a wave's chunks lie in one page");
+    constexpr int LPC = 7 + PSH - 3;                 // log2 of a page's chunks
+    static_assert((1 << LPC) == D * PS / 8 && LPC >= 6, "a wave's chunks lie in one page");
     typedef const __attribute__((address_space(4))) int32_t *constant_t;
     __shared__ __attribute__((aligned(16))) bf16_t Ks[KT * KP];
     __shared__ __attribute__((aligned(16))) bf16_t Vs[D * VP];
@@ -470,25 +473,25 @@ tree_wide_kernel(TreeArgs p, TreeSplit sp) {
         }
 }
 
-template <int D, int PSH, int W>
-int launch(const TreeArgs &a, int max_context, hipStream_t stream) {
-    const int G = a.heads / a.kv_heads, TQ = 32 * W / G;
+template <int PSH>
+int launch(const TreeArgs &a, hipStream_t stream) {
+    const int G = a.heads / a.kv_heads, TQ = ROWS / G;
     TreeSplit sp;
     sp.tiles = (a.max_nodes + TQ - 1) / TQ;
-    constexpr size_t part_bytes = (size_t)(4 * (D / 32) + 1) * W * kWave * 16;
+    constexpr size_t part_bytes = (size_t)(4 * (D / 32) + 1) * THREADS * 16;
     const long places = plan_places(a, 8 / W * compute_units(), 8, part_bytes, &sp);
     FLLM_REQUIRE(places <= 0x7fffffffL / 8, "tree_attention: grid too large");
     const long blocks = places * 8;
-    hipLaunchKernelGGL((tree_wide_kernel<D, PSH, W>), dim3((unsigned)blocks), dim3(W * kWave), 0, stream, a, sp);
+    hipLaunchKernelGGL(tree_wide_kernel<PSH>, dim3((unsigned)blocks), dim3(THREADS), 0, stream, a, sp);
     return fllm_check_launch("tree_attention");
 }
 
 }  // namespace
 
 // heads of 128, at most 64 query heads a key/value head, pages of 8 to 64 (tree_attention_mfma.hip has checked the rest)
-int fllm_tree_attention_wide(const TreeArgs &a, int max_context, hipStream_t stream) {
-    if (a.page_size == 8) return launch<128, 3, 4>(a, max_context, stream);
-    if (a.page_size == 16) return launch<128, 4, 4>(a, max_context, stream);
-    if (a.page_size == 32) return launch<128, 5, 4>(a, max_context, stream);
-    return launch<128, 6, 4>(a, max_context, stream);
+int fllm_tree_attention_wide(const TreeArgs &a, hipStream_t stream) {
+    if (a.page_size == 8) return launch<3>(a, stream);
+    if (a.page_size == 16) return launch<4>(a, stream);
+    if (a.page_size == 32) return launch<5>(a, stream);
+    return launch<6>(a, stream);
 }
