@@ -139,7 +139,9 @@ move_tokens_kernel(MoveArgs a) {
     }
 }
 
-constexpr int kPairs = 400;        // a launch carries that many pairs of pages in its arguments
+// A launch carries the pairs of pages in its arguments, which take 4 KiB at most with the 256 bytes that the compiler adds to them: as many as
+// that has room for, in steps of 64.  A launch costs the host about 4 us.
+constexpr int kPairs = 448;
 constexpr int kStores = 8;
 struct CopyArgs {
     char *base[kStores];
@@ -147,6 +149,7 @@ struct CopyArgs {
     int32_t layers[kStores];
     int32_t source[kPairs], target[kPairs];
 };
+static_assert(sizeof(CopyArgs) + 8 + 256 <= 4096 && sizeof(CopyArgs) + 8 + 256 + 64 * 8 > 4096, "the arguments of a launch");
 
 // blockIdx: (piece of a page, pair, layer and store).  A thread has four 16-byte pieces on their way.  Bound by memory: 400 pages of 16 layers
 // (419 MB in and out) 84 us, 5.0 TB/s, where one copy of 4 GiB gets 5.4; a page of 32 layers to seven others 6.9 us, the first read by one of

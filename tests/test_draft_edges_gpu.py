@@ -131,3 +131,14 @@ def test_a_request_that_ends_and_choices_that_are_refused(ops):
         want = plain_llama.forward(cfg, weights, prompts[r] + [newest[r], second[r], kept[i][1]])[-1]
         assert np.abs(row - want).max() <= TOL["float32"] * np.abs(want).max()
     runner.cache.check_invariants()
+
+
+@pytest.mark.parametrize("pairs", [63, 64, 399, 401, 447, 448, 449, 895, 897])
+def test_copies_at_the_edges_of_a_launch(ops, pairs):
+    store = torch.arange(2 * 2000 * 12, dtype=torch.float32).reshape(2, 2000, 12)
+    pages = torch.randperm(2000, generator=torch.Generator().manual_seed(pairs)).tolist()
+    source, target = pages[:pairs], pages[1000:1000 + pairs]
+    device = store.cuda()
+    ops.copy_pages((device,), source, target)
+    store[:, target] = store[:, source]
+    assert torch.equal(device.cpu(), store)
