@@ -14,8 +14,8 @@
 // What bounds it, with keys and values in memory: few tiles, the trips to memory that follow each other (a request of 8 nodes at 1,000
 // tokens of the 8B sizes 10.2 us, of which an empty launch is 2 and the parts' meeting 3); tiles as many as compute units, what a unit
 // gets from L2 (8 requests of up to 26 nodes at 2,048: four tiles read every key, 27 us, 8.5 TB/s of them); full tiles of heads of 64, the
-// exponentials and the other vector instructions (32 requests of up to 64 nodes at 6,144 127 us; with every key in L1 112); float32, the
-// matrix cores.  Blocks of twice the slots, or keys asked for two blocks ahead, need registers that two waves a SIMD do not have.
+// exponentials and the other vector instructions (32 requests of up to 64 nodes at 6,144 127 us; with every key in L1 112); float32,
+// trips to memory (4 requests of up to 13 nodes at 1,500 16.5 us: a wave has six blocks, and waits for 43 % of its time).  Blocks of twice the slots, or keys asked for two blocks ahead, need registers that two waves a SIMD do not have.
 // Slots that every row of the tile sees need no mask; a block that holds nodes, the end, the window's edge or a page that is none gets a
 // 64-bit mask a row.
 #include "common.h"

@@ -8,7 +8,7 @@
 // wants: the keys lie in LDS in the order that makes it so (bits 2 and 3 of a slot's number swapped).
 // Masks, what is not finite, and parts that several workgroups make of a tile's slots: as in tree_attention_mfma.hip.
 //
-// Two requests of 64 and 34 nodes at 32,768 and 28,593 tokens, 64 heads of 128 on 8: 146 us, 0.69 PFLOP/s.  Bound by the matrix
+// Two requests of 64 and 34 nodes at 32,768 and 28,593 tokens, 64 heads of 128 on 8: 142 us, 0.71 PFLOP/s (from memory 145).  Bound by the matrix
 // cores' rate on real numbers, 1.7 to 1.95 PFLOP/s (zeros: 2.5), and by what does not fit beside the products: with parts of the loop left out in
 // turn the weights took 28 us, LDS reads 12, stores to LDS 15.  One product behind the other on one sum takes 52 cycles instead of 32: the
 // scores take turns on two.  Operands are read from LDS six products ahead (written as a plain loop each is waited for: 178 us -> 164), the requests' slots are
