@@ -72,7 +72,7 @@ class TreeEntry:
 @dataclass
 class _Trees:
     """What a `step_tree` leaves for `keep_tree`."""
-    entries: List[TreeEntry]
+    req_ids: List[object]          # per entry
     order: List[int]               # segment -> entry
     ctx: StepContext
     most: int                      # nodes of the longest way from a root
@@ -196,7 +196,7 @@ class ModelRunner:
 
     def free_request(self, req_id) -> None:
         if self._tree is not None:                 # the other requests' trees are still there
-            self._tree.ended.update(i for i, e in enumerate(self._tree.entries) if e.req_id == req_id)
+            self._tree.ended.update(i for i, r in enumerate(self._tree.req_ids) if r == req_id)
         self.cache.free_request(req_id)
 
     def length(self, req_id) -> int:
@@ -317,14 +317,14 @@ class ModelRunner:
         """Leaves the last step's trees behind, if there are any."""
         trees, self._tree = self._tree, None
         if trees is not None:
-            live = [i for i in range(len(trees.entries)) if i not in trees.ended]
-            self._trim_trees([trees.entries[i] for i in live], [trees.held[i] for i in live])
+            live = [i for i in range(len(trees.req_ids)) if i not in trees.ended]
+            self._trim_trees([trees.req_ids[i] for i in live], [trees.held[i] for i in live])
 
-    def _trim_trees(self, entries: Sequence[TreeEntry], held: Sequence[int]) -> None:
+    def _trim_trees(self, req_ids: Sequence, held: Sequence[int]) -> None:
         """Gives the pages back that hold nothing but nodes; what was reserved for a request ahead of its tree stays."""
-        for e, tokens in zip(entries, held):
-            if self.cache.has_request(e.req_id):
-                self.cache.trim(e.req_id, max(self.cache.length(e.req_id), tokens))
+        for req_id, tokens in zip(req_ids, held):
+            if self.cache.has_request(req_id):
+                self.cache.trim(req_id, max(self.cache.length(req_id), tokens))
 
     def step_tree(self, entries: Sequence[TreeEntry]) -> torch.Tensor:
         """Runs trees of drafted tokens as one batch and returns float32 logits [nodes, vocab], entry by entry and node by node: each node's
@@ -360,7 +360,7 @@ class ModelRunner:
         try:
             logits = self._forward_trees(entries, rows, held)
         except BaseException:
-            self._trim_trees(entries, held)
+            self._trim_trees([e.req_id for e in entries], held)
             raise
         self.steps += 1
         self.rows_total += sum(len(e.tokens) for e in entries)
@@ -386,7 +386,7 @@ class ModelRunner:
         ctx.tree = TreeRows(row_slot=packed[:total], kept=packed[3 * total:], seen=torch.tensor(seen, dtype=torch.int64, device=self.device),
                             parents=packed[2 * total:3 * total], max_nodes=max(len(e.tokens) for e in entries))
         logits = self.model.forward(ctx)
-        self._tree = _Trees(list(entries), order, ctx, 1 + max(max(depths) for depths, _ in rows), held)
+        self._tree = _Trees([e.req_id for e in entries], order, ctx, 1 + max(max(depths) for depths, _ in rows), held)
         return logits
 
     def keep_tree(self, chosen: torch.Tensor) -> List[tuple]:
@@ -398,15 +398,15 @@ class ModelRunner:
         if self._tree is None:
             raise StepError("keep_tree follows a step_tree")
         trees = self._tree
-        entries, order, ctx, most = trees.entries, trees.order, trees.ctx, trees.most
-        rows = sum(len(e.tokens) for e in entries)
+        order, ctx, most = trees.order, trees.ctx, trees.most
+        rows = ctx.num_rows
         if chosen.shape != (rows,):
             raise StepError(f"{rows} nodes were computed, {tuple(chosen.shape)} tokens are given")
-        ops, S = self.rt.ops, len(entries)
+        ops, S = self.rt.ops, len(order)
         if order != list(range(S)):               # the logits have the order of the entries, the rows that of the segments
-            starts = [0]
-            for e in entries:
-                starts.append(starts[-1] + len(e.tokens))
+            sizes, starts = dict(zip(order, ctx.seg_rows)), [0]
+            for i in range(S):
+                starts.append(starts[-1] + sizes[i])
             chosen = chosen[torch.tensor([r for i in order for r in range(starts[i], starts[i + 1])], device=self.device)]
         path = torch.empty((S, most), dtype=torch.int32, device=self.device)
         ends = torch.empty((2, S), dtype=torch.int32, device=self.device)
@@ -427,7 +427,7 @@ class ModelRunner:
             if s in ended:
                 out[i] = ([], -1)
                 continue
-            self.cache.commit(entries[i].req_id, lengths[s])
+            self.cache.commit(trees.req_ids[i], lengths[s])
             out[i] = (walked[s][: lengths[s]], newest[s])
         self._leave_trees()
         return out

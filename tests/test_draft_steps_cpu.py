@@ -278,3 +278,22 @@ def test_requests_that_end_between_a_tree_and_what_is_kept_of_it(ended, again):
     runner.cache.check_invariants()
     with pytest.raises(StepError):
         runner.keep_tree(chosen)
+
+
+def test_a_caller_may_go_on_with_its_lists():
+    """The record of a step on trees is its own: lists that the caller changes meanwhile change nothing."""
+    runner, cfg, weights = runner_of("A")
+    vocab = cfg["vocab_size"]
+    prompts = {"a": tc.random_ids(20, vocab, 1), "b": tc.random_ids(7, vocab, 2)}
+    runner.step([StepEntry(r, p) for r, p in prompts.items()])
+    own = {r: own_tokens(cfg, weights, p, 3) for r, p in prompts.items()}
+    entries = [TreeEntry("a", own["a"][:1], [-1]), TreeEntry("b", [own["b"][0], 3, own["b"][1]], [-1, 0, 0])]
+    chosen = runner.step_tree(entries).argmax(dim=1).int()
+    entries[0].tokens.append(9), entries[1].tokens.clear(), entries[1].parents.clear()
+    entries[0].req_id = "c"
+    entries.pop()
+    assert runner.keep_tree(chosen) == [([0], own["a"][1]), ([0, 2], own["b"][2])]
+    got = runner.step([StepEntry("a", [own["a"][1]], want=(0,)), StepEntry("b", [own["b"][2]], want=(0,))])
+    next_logits(cfg, weights, prompts["a"] + own["a"][:2], got[0])
+    next_logits(cfg, weights, prompts["b"] + own["b"], got[1])
+    runner.cache.check_invariants()
